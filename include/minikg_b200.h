@@ -42,8 +42,12 @@ enum {
   MKG_DEV_BAD_REL = 16u,   /* relation id outside [0, R) */
   MKG_DEV_TIMEOUT = 32u,   /* a bounded wait inside a kernel gave up */
   MKG_DEV_TABLE_FULL = 64u, /* a message hash table ran out of slots (msg_bound too small) */
-  MKG_DEV_BAD_RULE_INDEX = 128u /* rule producer: relation outside [0, n) or query map outside [0, U) */
+  MKG_DEV_BAD_RULE_INDEX = 128u, /* rule producer: relation outside [0, n) or query map outside [0, U) */
+  MKG_DEV_BAD_TARGET = 256u /* log probabilities: a target outside [0, width) that is not -1 */
 };
+
+/* element types of the entry points that take more than fp32 */
+enum { MKG_F32 = 0, MKG_BF16 = 1, MKG_F16 = 2 };
 
 /* One direction of the reference CSR pair (fastlog_kernel.py:403-410 tuple order). */
 typedef struct mkg_csr_dir {
@@ -598,6 +602,47 @@ int mkg_rule_softmax_backward(const mkg_rule_params* p, const float* w_hops, con
                               const int64_t* query_ptr, const int64_t* query_perm,
                               float* grad_logits_u, void* workspace, size_t workspace_bytes,
                               unsigned* dev_err, mkg_stream stream);
+
+/* ------------------------------------------------------------ log probabilities of targets */
+
+enum { MKG_LOGPROB_TOPK_MAX = 32, MKG_LOGPROB_TARGETS_MAX = 1024 };
+
+/* Rows of logits x [rows, width] (rule logits over the channels, or scores over the entities).
+ * With z_j = x_j / tau over the row's candidates (every j, or those whose mask byte is not 0):
+ *   lse = log sum_j e^{z_j},  log p_j = z_j - lse,  entropy = -sum_j p_j log p_j. */
+typedef struct mkg_logprob_params {
+  int64_t rows;
+  int64_t width;           /* 1 .. 2^30 */
+  int64_t row_stride;      /* elements from one row of logits to the next */
+  int64_t mask_row_stride; /* bytes from one row of the mask to the next; 0: one row for all */
+  int64_t targets;         /* given columns per row, 0 .. MKG_LOGPROB_TARGETS_MAX */
+  int64_t topk;            /* alternatives per row, 0 .. MKG_LOGPROB_TOPK_MAX */
+  double tau;              /* > 0 */
+  int32_t dtype;           /* MKG_F32 / MKG_BF16 / MKG_F16, of the logits and their gradient */
+  int32_t reserved;
+} mkg_logprob_params;
+
+/* Writes logprobs [rows, targets] (log p of each target; a target of -1 is padding and gets 0,
+ * one that is no candidate gets -inf, one outside [-1, width) gets NaN and sets
+ * MKG_DEV_BAD_TARGET), entropy [rows], lse [rows], the topk largest candidates above -inf by
+ * logit (ties: the lowest column) as top_ids [rows, topk] / top_logprobs [rows, topk] (-1 / -inf
+ * where a row has fewer), and stats [rows, 2] for the backward (the row's largest logit and
+ * log2 of the sum of e^{z - its largest}).  A row without a candidate above -inf has lse -inf,
+ * entropy 0 and every log p -inf; a row with NaN or +inf among its candidates has NaN
+ * everywhere and no alternatives.  mask may be NULL. */
+size_t mkg_logprob_workspace_bytes(const mkg_logprob_params* p);
+int mkg_logprob_forward(const mkg_logprob_params* p, const void* logits, const uint8_t* mask, const int64_t* targets,
+                        float* logprobs, float* entropy, float* lse, int64_t* top_ids, float* top_logprobs,
+                        float* stats, void* workspace, size_t workspace_bytes, unsigned* dev_err, mkg_stream stream);
+
+/* Gradient of mkg_logprob_forward: grad [rows, width] (contiguous, the logits' type, overwritten)
+ * for the gradients of logprobs, entropy, lse and top_logprobs (each may be NULL: zero).  A column
+ * named more than once collects its gradients in order; columns that are no candidates and rows
+ * without one get 0. */
+int mkg_logprob_backward(const mkg_logprob_params* p, const void* logits, const uint8_t* mask, const int64_t* targets,
+                         const int64_t* top_ids, const float* entropy, const float* stats, const float* g_logprobs,
+                         const float* g_entropy, const float* g_lse, const float* g_top, void* grad,
+                         mkg_stream stream);
 
 #ifdef __cplusplus
 }

@@ -23,7 +23,10 @@ DEV_ERR_NAMES = {1: "frontier entry outside [B, L, E]", 2: "CSR column outside [
                  4: "fact id outside [0, T)", 8: "gradient key outside [B, L, E]",
                  16: "relation id outside its range", 32: "a bounded wait inside a kernel gave up",
                  64: "a message hash table ran out of slots (msg_bound too small)",
-                 128: "rule producer: relation outside [0, n) or query map outside [0, U)"}
+                 128: "rule producer: relation outside [0, n) or query map outside [0, U)",
+                 256: "log probabilities: a target outside [0, width)"}
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # MKG_F32, MKG_BF16, MKG_F16
+LOGPROB_TOPK_MAX, LOGPROB_TARGETS_MAX = 32, 1024  # MKG_LOGPROB_*_MAX
 
 vp = C.c_void_p
 i64 = C.c_int64
@@ -87,6 +90,11 @@ class SlabWindow(C.Structure):
 class RuleParams(C.Structure):
     _fields_ = [("n", i64), ("H", i64), ("L", i64), ("K", i64), ("U", i64), ("B", i64), ("tau", C.c_float),
                 ("reserved", i32)]
+
+
+class LogprobParams(C.Structure):
+    _fields_ = [("rows", i64), ("width", i64), ("row_stride", i64), ("mask_row_stride", i64), ("targets", i64),
+                ("topk", i64), ("tau", C.c_double), ("dtype", i32), ("reserved", i32)]
 
 
 P = C.POINTER
@@ -167,6 +175,9 @@ SIGNATURES = {
                                            vp, vp, vp, C.c_size_t, vp, vp]),
     "mkg_rule_softmax_forward": (C.c_int, [P(RuleParams), vp, vp, vp, vp, vp]),
     "mkg_rule_softmax_backward": (C.c_int, [P(RuleParams), vp, vp, vp, vp, vp, vp, C.c_size_t, vp, vp]),
+    "mkg_logprob_workspace_bytes": (C.c_size_t, [P(LogprobParams)]),
+    "mkg_logprob_forward": (C.c_int, [P(LogprobParams), vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, C.c_size_t, vp, vp]),
+    "mkg_logprob_backward": (C.c_int, [P(LogprobParams), vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp]),
 }
 
 _lib = None

@@ -195,3 +195,19 @@ MKG_API int mkg_cap_index_build(const mkg_graph* g, const mkg_adjacency* adj, co
                                 size_t ws_bytes, unsigned* err, mkg_stream st) {
   return mkg::cap_index_build(g, adj, index, ws, ws_bytes, err, S(st));
 }
+
+MKG_API size_t mkg_logprob_workspace_bytes(const mkg_logprob_params* p) { return mkg::logprob_workspace_bytes(p); }
+MKG_API int mkg_logprob_forward(const mkg_logprob_params* p, const void* logits, const uint8_t* mask,
+                                const int64_t* targets, float* logprobs, float* entropy, float* lse, int64_t* top_ids,
+                                float* top_logprobs, float* stats, void* ws, size_t ws_bytes, unsigned* err,
+                                mkg_stream st) {
+  return mkg::logprob_forward(p, logits, mask, targets, logprobs, entropy, lse, top_ids, top_logprobs, stats, ws,
+                              ws_bytes, err, S(st));
+}
+MKG_API int mkg_logprob_backward(const mkg_logprob_params* p, const void* logits, const uint8_t* mask,
+                                 const int64_t* targets, const int64_t* top_ids, const float* entropy,
+                                 const float* stats, const float* g_logprobs, const float* g_entropy,
+                                 const float* g_lse, const float* g_top, void* grad, mkg_stream st) {
+  return mkg::logprob_backward(p, logits, mask, targets, top_ids, entropy, stats, g_logprobs, g_entropy, g_lse, g_top,
+                               grad, S(st));
+}

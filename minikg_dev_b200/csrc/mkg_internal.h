@@ -84,4 +84,13 @@ int rule_softmax_backward(const mkg_rule_params* p, const float* w_hops, const f
                           const int64_t* query_ptr, const int64_t* query_perm, float* grad_logits_u, void* ws,
                           size_t ws_bytes, unsigned* err, cudaStream_t st);
 
+// mkg_logprob.cu
+size_t logprob_workspace_bytes(const mkg_logprob_params* p);
+int logprob_forward(const mkg_logprob_params* p, const void* logits, const uint8_t* mask, const int64_t* targets,
+                    float* logprobs, float* entropy, float* lse, int64_t* top_ids, float* top_logprobs, float* stats,
+                    void* ws, size_t ws_bytes, unsigned* err, cudaStream_t st);
+int logprob_backward(const mkg_logprob_params* p, const void* logits, const uint8_t* mask, const int64_t* targets,
+                     const int64_t* top_ids, const float* entropy, const float* stats, const float* g_logprobs,
+                     const float* g_entropy, const float* g_lse, const float* g_top, void* grad, cudaStream_t st);
+
 }  // namespace mkg
