@@ -644,6 +644,52 @@ int mkg_logprob_backward(const mkg_logprob_params* p, const void* logits, const 
                          const float* g_entropy, const float* g_lse, const float* g_top, void* grad,
                          mkg_stream stream);
 
+/* ------------------------------------------------------------ AdamW over many tensors */
+
+enum { MKG_ADAMW_BLOCK = 256 };
+
+typedef struct mkg_adamw_params {
+  double lr, beta1, beta2, eps, weight_decay;
+  const float* lr_device;  /* NULL, or one fp32 on the device that is read in place of lr */
+  int32_t param_dtype;     /* MKG_F32 / MKG_BF16 / MKG_F16 */
+  int32_t grad_dtype;
+  int32_t state_bits;      /* 32 or 8 */
+  int32_t reserved;
+} mkg_adamw_params;
+
+/* Moments of all tensors of an optimizer in two flat arrays of `total` values; each tensor starts
+ * on a multiple of MKG_ADAMW_BLOCK and what is left of its last block belongs to nobody (0).
+ * 32 bits: fp32 values, the scales may be NULL.  8 bits: one byte per value and per block of
+ * MKG_ADAMW_BLOCK a scale, a power of two s.  exp_avg: sign, 4 exponent and 3 mantissa bits (fp8
+ * e4m3) times s.  exp_avg_sq: code c stands for s 2^-33 c below 8, else s 2^(c/8 - 31) (1 + c%8 / 8);
+ * 255 is NaN.  Zeroed arrays stand for zero moments.  steps [tensors]: steps taken by each tensor.
+ * ticket: one word, 0 between calls; calls on one state must not run at the same time. */
+typedef struct mkg_adamw_state {
+  void* exp_avg;
+  void* exp_avg_sq;
+  float* exp_avg_scale;
+  float* exp_avg_sq_scale;
+  int64_t* steps;
+  unsigned* ticket;
+  int64_t total;
+  int64_t tensors;
+} mkg_adamw_state;
+
+/* One step of n tensors: host arrays of their device pointers, sizes, offsets into the moments and
+ * indexes into steps (each index at most once).  params are updated in place:
+ *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,  t = its step count + 1,
+ *   p = p (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * in fp32 (fp64 for moments in 8 bits, rounded once to what is held; the update takes m and v
+ * before that rounding).  Gradients that are not finite make the values they meet NaN. */
+int mkg_adamw_step(const mkg_adamw_params* p, const mkg_adamw_state* state, int64_t n, void* const* params,
+                   const void* const* grads, const int64_t* numel, const int64_t* offset, const int64_t* index,
+                   mkg_stream stream);
+
+/* Moments in 8 bits from fp32 [total] arrays and back (16-byte aligned); a second moment above 0 is
+ * never held as 0.  Packing what was unpacked changes nothing. */
+int mkg_adamw_pack(const mkg_adamw_state* state, const float* exp_avg, const float* exp_avg_sq, mkg_stream stream);
+int mkg_adamw_unpack(const mkg_adamw_state* state, float* exp_avg, float* exp_avg_sq, mkg_stream stream);
+
 #ifdef __cplusplus
 }
 #endif

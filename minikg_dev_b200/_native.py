@@ -27,6 +27,7 @@ DEV_ERR_NAMES = {1: "frontier entry outside [B, L, E]", 2: "CSR column outside [
                  256: "log probabilities: a target outside [0, width)"}
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # MKG_F32, MKG_BF16, MKG_F16
 LOGPROB_TOPK_MAX, LOGPROB_TARGETS_MAX = 32, 1024  # MKG_LOGPROB_*_MAX
+ADAMW_BLOCK = 256  # MKG_ADAMW_BLOCK
 
 vp = C.c_void_p
 i64 = C.c_int64
@@ -95,6 +96,17 @@ class RuleParams(C.Structure):
 class LogprobParams(C.Structure):
     _fields_ = [("rows", i64), ("width", i64), ("row_stride", i64), ("mask_row_stride", i64), ("targets", i64),
                 ("topk", i64), ("tau", C.c_double), ("dtype", i32), ("reserved", i32)]
+
+
+class AdamwParams(C.Structure):
+    _fields_ = [("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double),
+                ("weight_decay", C.c_double), ("lr_device", vp), ("param_dtype", i32), ("grad_dtype", i32),
+                ("state_bits", i32), ("reserved", i32)]
+
+
+class AdamwState(C.Structure):
+    _fields_ = [("exp_avg", vp), ("exp_avg_sq", vp), ("exp_avg_scale", vp), ("exp_avg_sq_scale", vp), ("steps", vp),
+                ("ticket", vp), ("total", i64), ("tensors", i64)]
 
 
 P = C.POINTER
@@ -177,6 +189,9 @@ SIGNATURES = {
     "mkg_rule_softmax_backward": (C.c_int, [P(RuleParams), vp, vp, vp, vp, vp, vp, C.c_size_t, vp, vp]),
     "mkg_logprob_workspace_bytes": (C.c_size_t, [P(LogprobParams)]),
     "mkg_logprob_forward": (C.c_int, [P(LogprobParams), vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, C.c_size_t, vp, vp]),
+    "mkg_adamw_step": (C.c_int, [P(AdamwParams), P(AdamwState), i64, vp, vp, vp, vp, vp, vp]),
+    "mkg_adamw_pack": (C.c_int, [P(AdamwState), vp, vp, vp]),
+    "mkg_adamw_unpack": (C.c_int, [P(AdamwState), vp, vp, vp]),
     "mkg_logprob_backward": (C.c_int, [P(LogprobParams), vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp]),
 }
 

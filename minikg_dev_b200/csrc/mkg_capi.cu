@@ -211,3 +211,16 @@ MKG_API int mkg_logprob_backward(const mkg_logprob_params* p, const void* logits
   return mkg::logprob_backward(p, logits, mask, targets, top_ids, entropy, stats, g_logprobs, g_entropy, g_lse, g_top,
                                grad, S(st));
 }
+
+MKG_API int mkg_adamw_step(const mkg_adamw_params* p, const mkg_adamw_state* state, int64_t n, void* const* params,
+                           const void* const* grads, const int64_t* numel, const int64_t* offset,
+                           const int64_t* index, mkg_stream st) {
+  return mkg::adamw_step(p, state, n, params, grads, numel, offset, index, S(st));
+}
+MKG_API int mkg_adamw_pack(const mkg_adamw_state* state, const float* exp_avg, const float* exp_avg_sq,
+                           mkg_stream st) {
+  return mkg::adamw_pack(state, exp_avg, exp_avg_sq, S(st));
+}
+MKG_API int mkg_adamw_unpack(const mkg_adamw_state* state, float* exp_avg, float* exp_avg_sq, mkg_stream st) {
+  return mkg::adamw_unpack(state, exp_avg, exp_avg_sq, S(st));
+}

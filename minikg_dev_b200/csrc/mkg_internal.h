@@ -93,4 +93,11 @@ int logprob_backward(const mkg_logprob_params* p, const void* logits, const uint
                      const int64_t* top_ids, const float* entropy, const float* stats, const float* g_logprobs,
                      const float* g_entropy, const float* g_lse, const float* g_top, void* grad, cudaStream_t st);
 
+// mkg_adamw.cu
+int adamw_step(const mkg_adamw_params* p, const mkg_adamw_state* state, int64_t n, void* const* params,
+               const void* const* grads, const int64_t* numel, const int64_t* offset, const int64_t* index,
+               cudaStream_t st);
+int adamw_pack(const mkg_adamw_state* state, const float* exp_avg, const float* exp_avg_sq, cudaStream_t st);
+int adamw_unpack(const mkg_adamw_state* state, float* exp_avg, float* exp_avg_sq, cudaStream_t st);
+
 }  // namespace mkg

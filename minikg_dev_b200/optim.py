@@ -1,0 +1,289 @@
+"""AdamW over many tensors in one launch, with the moments held in 32 or in 8 bits.
+
+``AdamW`` updates what a rule model trains: the producer's embeddings, LSTMs and linear layer (dozens
+of small tensors) and the facts' scores (one tensor of every fact).  It is a
+``torch.optim.Optimizer`` (parameter groups, learning-rate schedulers, ``zero_grad``, closures,
+step hooks), and a step is one ``mkg_adamw_step`` call per group and pair of element types, that is
+one launch for up to 800 tensors.  Nothing is copied to the device and the step counts live there, so
+a step can be captured in a CUDA graph (``proof.ProofRunner.capture(optimizer=...)`` does).
+
+``state_bits=8`` holds each moment in one byte and shares a power of two between 256 values: 2.03
+bytes a parameter in place of 8.  First moments have 4 significant bits, second moments 4 over 34
+binades; a second moment above 0 is never held as 0.  Sums are taken in fp64 and rounded once.
+"""
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import torch
+
+from . import _native as N
+
+_CODES = ("exp_avg_codes", "exp_avg_scale", "exp_avg_sq_codes", "exp_avg_sq_scale")
+
+
+class AdamW(torch.optim.Optimizer):
+    """``p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)`` on dense,
+    contiguous CUDA parameters (float32, bfloat16 or float16; gradients in any of the three), all on
+    one device.  Arithmetic is fp32 and each parameter is rounded to its type once.
+
+    ``lr`` is a number or a float32 CUDA tensor of one element; a captured step reads the tensor
+    at every replay, a number is kept as it was at capture.  Parameters without a gradient are left
+    alone and their step count with them.  Not offered: sparse or complex gradients, ``amsgrad``,
+    ``maximize``; non-contiguous parameters and parameters that share memory are refused.  Two steps
+    of one optimizer must not run at the same time.
+    """
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, *,
+                 state_bits: int = 32):
+        if state_bits not in (8, 32):
+            raise ValueError(f"AdamW: state_bits must be 8 or 32, got {state_bits}")
+        self.state_bits = int(state_bits)
+        self._plan = []     # per group: (numel, offset, index) int64 arrays over its parameters
+        self._buffers = {}  # flat moments, scales, step counts, the ticket word
+        self._total = self._tensors = 0
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
+
+    # ------------------------------------------------------------------ parameters and their state
+    def _check_group(self, group) -> None:
+        lr, (b1, b2), eps, wd = group["lr"], group["betas"], group["eps"], group["weight_decay"]
+        if isinstance(lr, torch.Tensor):
+            if lr.numel() != 1 or lr.dtype != torch.float32 or not lr.is_cuda:
+                raise ValueError("AdamW: a tensor lr must be one float32 value on the parameters' device")
+        elif not (lr >= 0.0 and math.isfinite(lr)):
+            raise ValueError(f"AdamW: lr must be finite and not negative, got {lr}")
+        if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0):
+            raise ValueError(f"AdamW: betas must be in [0, 1), got {(b1, b2)}")
+        if not (eps >= 0.0 and wd >= 0.0 and math.isfinite(eps) and math.isfinite(wd)):
+            raise ValueError(f"AdamW: eps and weight_decay must be finite and not negative, got {eps}, {wd}")
+
+    def add_param_group(self, param_group) -> None:
+        before = len(self.param_groups)
+        super().add_param_group(param_group)
+        try:
+            group = self.param_groups[-1]
+            self._check_group(group)
+            for p in group["params"]:
+                if p.dtype not in N.DTYPES:
+                    raise TypeError(f"AdamW: parameters must be float32, bfloat16 or float16, got {p.dtype}")
+                if p.layout != torch.strided or not p.is_contiguous():
+                    raise ValueError("AdamW: parameters must be dense and contiguous")
+            every = [p for g in self.param_groups for p in g["params"]]
+            for p in group["params"]:
+                N.require_cuda(p, "AdamW parameters")
+                if p.device != every[0].device:
+                    raise ValueError(f"AdamW: parameters on {every[0].device} and {p.device}")
+            spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in every if p.numel())
+            if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+                raise ValueError("AdamW: parameters share memory")
+            if isinstance(group["lr"], torch.Tensor) and every and group["lr"].device != every[0].device:
+                raise ValueError("AdamW: a tensor lr must be one float32 value on the parameters' device")
+        except Exception:
+            del self.param_groups[before:]
+            raise
+        self._extend(group["params"])
+
+    def _extend(self, params) -> None:
+        """Room in the flat buffers for one more group; a graph captured before has to be captured again."""
+        numel = np.array([p.numel() for p in params], dtype=np.int64)
+        room = -(-numel // N.ADAMW_BLOCK) * N.ADAMW_BLOCK
+        offset = self._total + np.concatenate([[0], np.cumsum(room)[:-1]]).astype(np.int64)
+        index = self._tensors + np.arange(len(params), dtype=np.int64)
+        self._plan.append((numel, offset, index))
+        self._total += int(room.sum())
+        self._tensors += len(params)
+        if params:
+            self._allocate(params[0].device)
+
+    def _allocate(self, dev) -> None:
+        held = torch.float32 if self.state_bits == 32 else torch.uint8
+        want = {"exp_avg": (self._total, held), "exp_avg_sq": (self._total, held),
+                "steps": (self._tensors, torch.int64), "ticket": (1, torch.int32)}
+        if self.state_bits == 8:
+            want |= {k: (self._total // N.ADAMW_BLOCK, torch.float32) for k in ("exp_avg_scale", "exp_avg_sq_scale")}
+        old, self._buffers = self._buffers, {}
+        for name, (n, dtype) in want.items():
+            b = torch.zeros(max(n, 1), dtype=dtype, device=dev)
+            if name in old and name != "ticket":
+                b[:old[name].numel()].copy_(old[name])
+            self._buffers[name] = b
+        self._views()
+
+    def _views(self) -> None:
+        """``state[p]``: each parameter's part of the flat buffers."""
+        b = self._buffers
+        for group, (numel, offset, index) in zip(self.param_groups, self._plan):
+            for p, n, at, i in zip(group["params"], numel.tolist(), offset.tolist(), index.tolist()):
+                if self.state_bits == 32:
+                    moments = {k: b[k][at:at + n].view(p.shape) for k in ("exp_avg", "exp_avg_sq")}
+                else:
+                    blocks = slice(at // N.ADAMW_BLOCK, -(-(at + n) // N.ADAMW_BLOCK))
+                    moments = dict(zip(_CODES, (b["exp_avg"][at:at + n].view(p.shape), b["exp_avg_scale"][blocks],
+                                                b["exp_avg_sq"][at:at + n].view(p.shape),
+                                                b["exp_avg_sq_scale"][blocks])))
+                self.state[p] = {"step": b["steps"][i], **moments}
+
+    def _state_struct(self, buffers=None) -> N.AdamwState:
+        b = buffers or self._buffers
+        return N.AdamwState(b["exp_avg"].data_ptr(), b["exp_avg_sq"].data_ptr(), N.ptr(b.get("exp_avg_scale")),
+                            N.ptr(b.get("exp_avg_sq_scale")), b["steps"].data_ptr(), b["ticket"].data_ptr(),
+                            self._total, self._tensors)
+
+    def __getstate__(self):
+        return self.__dict__.copy()
+
+    # ------------------------------------------------------------------ the step
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        if len(self._plan) != len(self.param_groups):
+            raise RuntimeError("AdamW: parameter groups are added with add_param_group")
+        for group, plan in zip(self.param_groups, self._plan):
+            params = group["params"]
+            if len(params) != len(plan[0]):
+                raise RuntimeError("AdamW: a group's parameters changed after it was added")
+            grads = [p.grad for p in params]
+            kinds = {(p.dtype, None if g is None else g.dtype) for p, g in zip(params, grads)}
+            if len(kinds) == 1 and None not in next(iter(kinds)):
+                self._launch(group, params, grads, *plan)
+                continue
+            for kind in sorted(kinds, key=str):
+                at = [i for i, (p, g) in enumerate(zip(params, grads)) if g is not None and (p.dtype, g.dtype) == kind]
+                if at:
+                    self._launch(group, [params[i] for i in at], [grads[i] for i in at], *(a[at] for a in plan))
+        return loss
+
+    def load_kernels(self) -> None:
+        """Loads what ``step`` launches with the present gradients, without a step: before a capture."""
+        for group, plan in zip(self.param_groups, self._plan):
+            seen = set()
+            for p in group["params"]:
+                if p.grad is None or (p.dtype, p.grad.dtype) in seen:
+                    continue
+                seen.add((p.dtype, p.grad.dtype))
+                none = np.zeros(len(group["params"]), dtype=np.int64)
+                self._call(group, p.dtype, p.grad.dtype, none, none, none, none, none)
+
+    def _call(self, group, p_dtype, g_dtype, p_at, g_at, numel, offset, index) -> None:
+        self._check_group(group)
+        dev, lr = self._buffers["steps"].device, group["lr"]
+        on_device = isinstance(lr, torch.Tensor)
+        b1, b2 = group["betas"]
+        hyper = N.AdamwParams(0.0 if on_device else float(lr), float(b1), float(b2), float(group["eps"]),
+                              float(group["weight_decay"]), lr.data_ptr() if on_device else None, N.DTYPES[p_dtype],
+                              N.DTYPES[g_dtype], self.state_bits, 0)
+        with torch.cuda.device(dev):
+            N.check(N.load().mkg_adamw_step(hyper, self._state_struct(), len(numel), p_at.ctypes.data, g_at.ctypes.data,
+                                            numel.ctypes.data, offset.ctypes.data, index.ctypes.data,
+                                            N.stream_handle(dev)), "adamw_step")
+
+    def _launch(self, group, params, grads, numel, offset, index) -> None:
+        dev = self._buffers["steps"].device
+        n, dtypes = len(params), (params[0].dtype, grads[0].dtype)
+        if dtypes[0] not in N.DTYPES or dtypes[1] not in N.DTYPES:
+            raise TypeError(f"AdamW: parameters of {dtypes[0]} with gradients of {dtypes[1]}")
+        if not all(g.layout == torch.strided for g in grads):
+            raise RuntimeError("AdamW: gradients must be dense")
+        if not all(map(torch.Tensor.is_contiguous, grads)):
+            grads = [g.contiguous() for g in grads]
+        own = numel.tolist()
+        if (list(map(torch.Tensor.numel, params)) != own or list(map(torch.Tensor.numel, grads)) != own
+                or not all(map(torch.Tensor.is_contiguous, params))):
+            raise RuntimeError("AdamW: a parameter changed its size or layout, or its gradient has another size")
+        where = set(map(torch.Tensor.get_device, params))
+        where.update(map(torch.Tensor.get_device, grads))
+        if where != {dev.index}:
+            raise RuntimeError(f"AdamW: parameters and gradients must be on {dev}")
+        p_at = np.fromiter(map(torch.Tensor.data_ptr, params), np.int64, n)
+        g_at = np.fromiter(map(torch.Tensor.data_ptr, grads), np.int64, n)
+        self._call(group, *dtypes, p_at, g_at, numel, offset, index)
+        torch.autograd.graph.increment_version(params)
+
+    # ------------------------------------------------------------------ the moments
+    def moments(self) -> tuple[torch.Tensor, torch.Tensor]:
+        """(exp_avg, exp_avg_sq) of every parameter, in the order of the groups, as flat fp32 arrays in
+        which each parameter starts on a multiple of 256 values: the optimizer's own buffers, or the
+        values that the 8-bit ones stand for."""
+        if not self._buffers:
+            return torch.empty(0), torch.empty(0)
+        if self.state_bits == 32:
+            return self._buffers["exp_avg"][:self._total], self._buffers["exp_avg_sq"][:self._total]
+        return self._unpacked(self._buffers)
+
+    def _unpacked(self, buffers):
+        dev = buffers["steps"].device
+        m, v = (torch.empty(max(self._total, 1), dtype=torch.float32, device=dev) for _ in range(2))
+        with torch.cuda.device(dev):
+            N.check(N.load().mkg_adamw_unpack(self._state_struct(buffers), m.data_ptr(), v.data_ptr(),
+                                              N.stream_handle(dev)), "adamw_unpack")
+        return m[:self._total], v[:self._total]
+
+    def load_state_dict(self, state_dict) -> None:
+        """Loads a state dict of this class or of ``torch.optim.AdamW`` into the buffers in place: moments
+        given as fp32 values are rounded to what 8 bits hold, moments given in 8 bits are read as the
+        values they stand for.  Parameters without an entry start anew."""
+        groups = state_dict["param_groups"]
+        if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
+            raise ValueError("AdamW: the state dict has other parameter groups")
+        for have, new in zip(self.param_groups, groups):
+            merged = {k: new[k] if k in new else v for k, v in have.items() if k != "params"}
+            if isinstance(have["lr"], torch.Tensor):
+                merged["lr"] = have["lr"]  # a captured step reads this tensor
+            merged["betas"] = tuple(merged["betas"])
+            self._check_group(merged)
+        if not self._buffers:
+            return
+        entries = []
+        for group, new, plan in zip(self.param_groups, groups, self._plan):
+            for p, key, n, at, i in zip(group["params"], new["params"], *(a.tolist() for a in plan)):
+                e = state_dict["state"].get(key)
+                if e is None:
+                    continue
+                if "exp_avg" not in e and _CODES[0] not in e:
+                    raise ValueError("AdamW: a state dict entry without moments")
+                if e["exp_avg" if "exp_avg" in e else _CODES[0]].numel() != n:
+                    raise ValueError("AdamW: a state dict entry of another size")
+                entries.append((e, n, at, i))
+        dev = self._buffers["steps"].device
+        m, v = (torch.zeros(max(self._total, 1), dtype=torch.float32, device=dev) for _ in range(2))
+        codes = {k: torch.zeros(max(self._total, 1), dtype=torch.uint8, device=dev) for k in ("exp_avg", "exp_avg_sq")}
+        codes |= {k: torch.zeros(max(self._total // N.ADAMW_BLOCK, 1), device=dev) for k in _CODES[1::2]}
+        codes |= {k: self._buffers[k] for k in ("steps", "ticket")}
+        any_codes = False
+        for e, n, at, _ in entries:
+            if "exp_avg" in e:
+                continue
+            any_codes = True
+            blocks = slice(at // N.ADAMW_BLOCK, -(-(at + n) // N.ADAMW_BLOCK))
+            codes["exp_avg"][at:at + n].copy_(e[_CODES[0]].reshape(-1))
+            codes["exp_avg_scale"][blocks].copy_(e[_CODES[1]])
+            codes["exp_avg_sq"][at:at + n].copy_(e[_CODES[2]].reshape(-1))
+            codes["exp_avg_sq_scale"][blocks].copy_(e[_CODES[3]])
+        if any_codes:
+            m, v = (x.contiguous() for x in self._unpacked(codes))
+        steps = torch.zeros(max(self._tensors, 1), dtype=torch.int64)
+        for e, n, at, i in entries:
+            steps[i] = int(e["step"])
+            if "exp_avg" in e:
+                m[at:at + n].copy_(e["exp_avg"].reshape(-1))
+                v[at:at + n].copy_(e["exp_avg_sq"].reshape(-1))
+        self._buffers["steps"].copy_(steps)
+        if self.state_bits == 32:
+            self._buffers["exp_avg"][:self._total].copy_(m[:self._total])
+            self._buffers["exp_avg_sq"][:self._total].copy_(v[:self._total])
+        else:
+            with torch.cuda.device(dev):
+                N.check(N.load().mkg_adamw_pack(self._state_struct(), m.data_ptr(), v.data_ptr(),
+                                                N.stream_handle(dev)), "adamw_pack")
+        for have, new in zip(self.param_groups, groups):
+            for k in have:
+                if k == "params" or k not in new:
+                    continue
+                if k == "lr" and isinstance(have["lr"], torch.Tensor):
+                    have["lr"].copy_(torch.as_tensor(new["lr"]).reshape(have["lr"].shape))
+                else:
+                    have[k] = tuple(new[k]) if k == "betas" else new[k]

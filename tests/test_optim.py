@@ -1,0 +1,512 @@
+"""optim.AdamW against its definition in float64, what 8 bits hold against a table of the held values,
+the bookkeeping around a step, and its refusals.
+
+Tolerances, from the arithmetic, with u = 2^-24 (fp32 rounds by u relative):
+* m = fma(b1, m, a1 g): b1, a1 and the product are rounded, then the sum: 3 u (|b1 m| + |a1 g|);
+  v likewise with one more product: 5 u v (all terms positive);
+* the update s m / (sqrt(v) r + eps): s, r, the root, the fma, the division and the product: 8 u on
+  top of what m and v carry (m's 3 u is of |b1 m| + |a1 g|), then the sum with p (1 - lr wd): 2 u |p|
+  and the rounding to the parameter's type, half a step: eps / 2.
+Moments in 8 bits are sums in fp64 rounded once: they have to be the nearest held value exactly.
+"""
+from __future__ import annotations
+
+import copy
+import math
+
+import pytest
+import torch
+
+from minikg_dev_b200 import _native as N
+from minikg_dev_b200.optim import AdamW
+
+gpu = pytest.mark.gpu
+U = 2.0 ** -24
+BLOCK = 256
+DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+
+
+# ------------------------------------------------------------------ what 8 bits hold, by table
+def first_table():
+    c = torch.arange(127, dtype=torch.float64)
+    return torch.where(c < 8, c * 2.0 ** -9, (1 + c % 8 / 8) * 2.0 ** (torch.div(c, 8, rounding_mode="floor") - 7))
+
+
+def second_table():
+    c = torch.arange(255, dtype=torch.float64)
+    return torch.where(c < 8, c * 2.0 ** -33, (1 + c % 8 / 8) * 2.0 ** (torch.div(c, 8, rounding_mode="floor") - 31))
+
+
+def nearest(table, y):
+    """Codes of the nearest table values to y >= 0 (largest at most), ties to the even code."""
+    hi = torch.searchsorted(table, y).clamp_max(len(table) - 1)
+    lo = (hi - 1).clamp_min(0)
+    up, down = table[hi] - y, y - table[lo]
+    return torch.where((up < down) | ((up == down) & (hi % 2 == 0)), hi, lo)
+
+
+def hold(x, table, low):
+    """(values, codes, scales) that 8 bits hold of one tensor's x >= 0, block by block."""
+    n = x.numel()
+    pad = torch.zeros(-(-n // BLOCK) * BLOCK, dtype=torch.float64)
+    pad[:n] = x.reshape(-1).cpu()
+    b = pad.view(-1, BLOCK)
+    scales = []
+    for a in b.amax(1).tolist():
+        e = low
+        while a > float(table[-1]) * 2.0 ** e:
+            e += 1
+        scales.append(2.0 ** e)
+    s = torch.tensor(scales, dtype=torch.float64)[:, None]
+    codes = nearest(table, b / s)
+    return (table[codes] * s).view(-1)[:n], codes.view(-1)[:n], s[:, 0]
+
+
+def held(m, v):
+    mm, _, _ = hold(m.abs(), first_table(), -120)
+    vv, codes, s = hold(v, second_table(), -90)
+    least = second_table()[1] * s.repeat_interleave(BLOCK)[:vv.numel()]
+    vv = torch.where((codes == 0) & (v.reshape(-1).cpu() > 0), least, vv)
+    return (torch.sign(m.reshape(-1).cpu()) * mm).view(m.shape), vv.view(v.shape)
+
+
+def definition(p, g, m, v, t, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, wd=0.01):
+    p, g, m, v = (x.double().cpu() for x in (p, g, m, v))
+    b1, b2 = betas
+    size = b1 * m.abs() + (1 - b1) * g.abs()
+    m = b1 * m + (1 - b1) * g
+    v = b2 * v + (1 - b2) * (g * g)
+    step = lr / (1 - b1 ** t)
+    below = v.sqrt() / math.sqrt(1 - b2 ** t) + eps
+    return p * (1 - lr * wd) - step * m / below, m, v, (size, step / below)
+
+
+def close(got, want, tol, what):
+    off = (got.double().cpu() - want).abs()
+    assert bool((off <= tol).all()), f"{what}: {float((off / tol.clamp_min(1e-300)).max())} times the tolerance"
+
+
+def make(sizes, dtype, grad_dtype, seed=0, shift=0):
+    """Parameters (views `shift` elements into their storage) with gradients."""
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    out = []
+    for n in sizes:
+        n = n if isinstance(n, tuple) else (n,)
+        k = math.prod(n)
+        flat = torch.randn(k + shift, generator=gen, device="cuda").to(dtype)
+        p = torch.nn.Parameter(flat[shift:].view(n))
+        size = 10.0 ** float(torch.rand((), generator=gen, device="cuda") * 6 - 5)
+        g = (torch.randn(k + shift, generator=gen, device="cuda") * size)
+        g[torch.rand(k + shift, generator=gen, device="cuda") < 0.1] = 0
+        g = g.to(grad_dtype)[shift:].view(n)
+        p.grad = g if grad_dtype == dtype else None
+        out.append((p, g))
+    return out
+
+
+def set_grads(pairs):
+    """Gradients of another type than the parameter's, as a program that accumulates in fp32 has them."""
+    for p, g in pairs:
+        if p.grad is None:
+            if hasattr(p, "grad_dtype"):
+                p.grad_dtype = g.dtype
+            p.grad = g
+
+
+SIZES = (1, 3, 4, 255, 256, 257, 2047, 2048, 2049, (33, 65), 10000, (1, 1), 0)
+
+
+@gpu
+@pytest.mark.parametrize("bits", (32, 8))
+@pytest.mark.parametrize("shift", (0, 1, 2))
+@pytest.mark.parametrize("dtype, grad_dtype", [(a, b) for a in DTYPES for b in (a, torch.float32)][1:])
+def test_steps(dtype, grad_dtype, shift, bits):
+    pairs = make(SIZES, dtype, grad_dtype, seed=shift, shift=shift)
+    set_grads(pairs)
+    params = [p for p, _ in pairs]
+    opt = AdamW(params, lr=1e-2, weight_decay=0.1, state_bits=bits)
+    sizes = [p.numel() for p in params]
+    starts = [0]
+    for n in sizes:
+        starts.append(starts[-1] + -(-n // BLOCK) * BLOCK)
+    for t in (1, 2, 3):
+        before = [p.detach().clone() for p in params]
+        fm, fv = (x.clone() for x in opt.moments())
+        opt.step()
+        gm, gv = opt.moments()
+        for i, (p, g) in enumerate(pairs):
+            n, at = sizes[i], starts[i]
+            m0, v0 = fm[at:at + n].view(p.shape), fv[at:at + n].view(p.shape)
+            want, m, v, (size, rate) = definition(before[i], g, m0, v0, t, lr=1e-2, wd=0.1)
+            m_tol, v_tol = 3 * U * size + 1e-45, 5 * U * v + 1e-45
+            eps = torch.finfo(dtype).eps
+            tiny = torch.finfo(dtype).smallest_normal * eps  # a subnormal's step
+            tol = rate * (3 * U * size + 8 * U * (m.abs() + size)) + 4 * U * want.abs() + 4 * U * before[i].double().cpu().abs()
+            # v's share: its root is off by half its relative error (and by what an fp32 subnormal v loses)
+            tol += rate * m.abs() * 3 * U
+            close(p, want, tol + eps / 2 * (want.abs() + tol) + tiny, f"step {t} parameter {i}")
+            if bits == 32:
+                close(gm[at:at + n].view(p.shape), m, m_tol, f"step {t} m {i}")
+                close(gv[at:at + n].view(p.shape), v, v_tol, f"step {t} v {i}")
+            elif n:
+                hm, hv = held(m, v)
+                assert torch.equal(gm[at:at + n].view(p.shape).double().cpu(), hm), f"step {t} held m {i}"
+                assert torch.equal(gv[at:at + n].view(p.shape).double().cpu(), hv), f"step {t} held v {i}"
+            # what is left of the last block stays 0
+            assert not gm[at + n:starts[i + 1]].any() and not gv[at + n:starts[i + 1]].any()
+            assert int(opt.state[p]["step"]) == (t if n else 0)
+
+
+@gpu
+@pytest.mark.parametrize("bits", (32, 8))
+def test_many_tensors_take_several_launches(bits):
+    sizes = [1 + (i * 37) % 301 for i in range(1700)]
+    pairs = make(sizes, torch.float32, torch.float32, seed=4)
+    before = [p.detach().clone() for p, _ in pairs]
+    opt = AdamW([p for p, _ in pairs], state_bits=bits)
+    opt.step()
+    for i in range(0, 1700, 7):
+        p, g = pairs[i]
+        zero = torch.zeros_like(g)
+        want, m, v, (size, rate) = definition(before[i], g, zero, zero, 1)
+        close(p, want, 16 * U * (rate * size + want.abs() + before[i].double().cpu().abs()), f"tensor {i}")
+        assert int(opt.state[p]["step"]) == 1
+    assert int(opt._buffers["ticket"]) == 0
+
+
+@gpu
+def test_against_torch():
+    torch.manual_seed(0)
+    model = torch.nn.Sequential(torch.nn.Linear(37, 51), torch.nn.LSTM(51, 16, bidirectional=True)).cuda()
+    twin = copy.deepcopy(model)
+    a = AdamW(model.parameters(), lr=3e-3, weight_decay=0.05)
+    b = torch.optim.AdamW(twin.parameters(), lr=3e-3, weight_decay=0.05)
+    sched = [torch.optim.lr_scheduler.ExponentialLR(o, 0.9) for o in (a, b)]
+    for i in range(20):
+        x = torch.randn(5, 37, device="cuda")
+        for net, opt, s in ((model, a, sched[0]), (twin, b, sched[1])):
+            opt.zero_grad()
+            net[1](net[0](x))[0].square().sum().backward()
+            if net is twin:  # the same gradients for both: only the update is compared
+                for p, q in zip(model.parameters(), twin.parameters()):
+                    q.grad.copy_(keep[p])
+            else:
+                keep = {p: p.grad.clone() for p in model.parameters()}
+            opt.step()
+            s.step()
+    for p, q in zip(model.parameters(), twin.parameters()):
+        # 20 steps of at most lr each, 16 u off a step, and the parameter's own roundings
+        assert float((p - q).abs().max()) <= 20 * (16 * U * 3e-3 * 4 + 2 * U * float(q.abs().max()))
+
+
+@gpu
+@pytest.mark.parametrize("bits", (32, 8))
+def test_groups_missing_gradients_and_rates(bits):
+    pairs = make((300, 40, 500, 7), torch.float32, torch.float32)
+    (p0, g0), (p1, _), (p2, g2), (p3, g3) = pairs
+    p1.grad = None
+    opt = AdamW([{"params": [p0, p1]}, {"params": [p2], "lr": 0.5, "betas": (0.5, 0.6), "weight_decay": 0.0}],
+                lr=0.1, eps=1e-3, state_bits=bits)
+    opt.step()
+    opt.add_param_group({"params": [p3], "lr": 0.25})
+    before = [p.detach().clone() for p, _ in pairs]
+    m0, v0 = (x.clone() for x in opt.moments())
+    opt.step()
+    assert torch.equal(p1, before[1]) and [int(opt.state[p]["step"]) for p, _ in pairs] == [2, 0, 2, 1]
+    for i, p, g, at, t, kw in ((0, p0, g0, 0, 2, dict(lr=0.1)), (2, p2, g2, 768, 2, dict(lr=0.5, betas=(0.5, 0.6), wd=0.0)),
+                               (3, p3, g3, 1280, 1, dict(lr=0.25))):
+        want, *_, (size, rate) = definition(before[i], g, m0[at:at + p.numel()], v0[at:at + p.numel()], t, eps=1e-3, **kw)
+        close(p, want, 16 * U * (rate * size + want.abs() + before[i].double().cpu().abs()), f"parameter {i}")
+
+
+@gpu
+def test_mixed_types_in_one_group():
+    pairs = make((100, 300), torch.float32, torch.float32) + make((200, 50), torch.bfloat16, torch.bfloat16)
+    opt = AdamW([p for p, _ in pairs])
+    before = [p.detach().clone() for p, _ in pairs]
+    opt.step()
+    for (p, g), b in zip(pairs, before):
+        zero = torch.zeros_like(g)
+        want, *_ = definition(b, g, zero, zero, 1)
+        close(p, want, (torch.finfo(p.dtype).eps / 2 + 32 * U) * (want.abs() + 2e-3), str(p.dtype))
+
+
+@gpu
+def test_gradients_of_other_layouts_and_shared_ones():
+    p = torch.nn.Parameter(torch.randn(30, 50, device="cuda"))
+    q = torch.nn.Parameter(p.detach().clone())
+    g = torch.randn(50, 30, device="cuda")
+    p.grad, q.grad = g.t(), g.t().contiguous()
+    AdamW([p]).step()
+    AdamW([q]).step()
+    assert torch.equal(p, q)
+    a, b = (torch.nn.Parameter(torch.ones(5, device="cuda")) for _ in range(2))
+    a.grad = b.grad = torch.arange(5.0, device="cuda")
+    AdamW([a, b]).step()
+    assert torch.equal(a, b)
+
+
+@gpu
+def test_not_finite_gradients():
+    for bits in (32, 8):
+        p = torch.nn.Parameter(torch.ones(600, device="cuda"))
+        p.grad = torch.full((600,), 0.5, device="cuda")
+        p.grad[3], p.grad[300] = math.nan, math.inf
+        opt = AdamW([p], state_bits=bits)
+        opt.step()
+        bad = torch.zeros(600, dtype=torch.bool, device="cuda")
+        bad[3] = bad[300] = True
+        assert torch.equal(torch.isnan(p), bad)
+        m, v = opt.moments()
+        assert not torch.isfinite(m[:600])[bad].any() and not torch.isfinite(v[:600])[bad].any()
+        assert torch.isfinite(m[:600])[~bad].all() and torch.isfinite(v[:600])[~bad].all()
+
+
+@gpu
+def test_extremes_in_8_bits():
+    """Second moments down to the smallest stay above 0; those too large to square stay finite."""
+    p = torch.nn.Parameter(torch.zeros(1024, device="cuda"))
+    g = torch.zeros(1024, device="cuda")
+    g[:256] = 2.0 ** -torch.arange(256, device="cuda").float().clamp_max(140)
+    g[256:512] = 1e-30
+    g[512] = 1e38
+    g[513:768] = 1.0
+    p.grad = g
+    opt = AdamW([p], lr=0.0, state_bits=8)
+    opt.step()
+    m, v = opt.moments()
+    gd = g.double().cpu()
+    hm, _ = held((1 - 0.9) * gd, torch.zeros(1024, dtype=torch.float64))
+    assert torch.equal(m.double().cpu(), hm)
+    nonzero = gd != 0
+    assert bool((v.cpu()[nonzero] > 0).all()) and not v.cpu()[~nonzero].any() and torch.isfinite(v).all()
+
+
+@gpu
+@pytest.mark.parametrize("start", (torch.float32, "codes", "torch"))
+@pytest.mark.parametrize("bits", (32, 8))
+def test_state_dicts(start, bits):
+    pairs = make((700, (3, 5), 1000), torch.float32, torch.float32, seed=2)
+    params = [p for p, _ in pairs]
+    if start == "torch":
+        src = torch.optim.AdamW(params, lr=0.02)
+    else:
+        src = AdamW(params, lr=0.02, state_bits=8 if start == "codes" else 32)
+    for _ in range(3):
+        src.step()
+    saved = copy.deepcopy(src.state_dict())
+    twins = [torch.nn.Parameter(p.detach().clone()) for p in params]
+    for q, (_, g) in zip(twins, pairs):
+        q.grad = g.clone()
+    dst = AdamW(twins, lr=0.7, state_bits=bits)
+    before = dst._buffers["exp_avg"].data_ptr()
+    dst.load_state_dict(saved)
+    assert dst._buffers["exp_avg"].data_ptr() == before  # in place: captured steps stay valid
+    assert dst.param_groups[0]["lr"] == 0.02 and [int(dst.state[q]["step"]) for q in twins] == [3, 3, 3]
+    m, v = (x.clone() for x in dst.moments())
+    at = 0
+    for p, q in zip(params, twins):
+        n = p.numel()
+        if start == "codes":
+            sm, sv = (x[at:at + n] for x in src.moments())
+        else:
+            sm, sv = src.state[p]["exp_avg"].reshape(-1), src.state[p]["exp_avg_sq"].reshape(-1)
+        if bits == 8 and start != "codes":
+            sm, sv = (x.float().cuda() for x in held(sm, sv))
+        assert torch.equal(m[at:at + n], sm) and torch.equal(v[at:at + n], sv)
+        at += -(-n // BLOCK) * BLOCK
+    if start == "codes" and bits == 8 or start is torch.float32 and bits == 32:
+        src.step()
+        dst.step()
+        for p, q in zip(params, twins):
+            assert torch.equal(p, q)
+        again = copy.deepcopy(dst.state_dict())  # there and back
+        dst.load_state_dict(again)
+        for key, a in again["state"].items():
+            for name, x in a.items():
+                assert torch.equal(x, dst.state_dict()["state"][key][name]), name
+    copied = copy.deepcopy(dst)
+    copied.param_groups[0]["params"][0].grad = twins[0].grad.clone()
+    copied.step()
+    assert int(copied.state[copied.param_groups[0]["params"][0]]["step"]) == int(dst.state[twins[0]]["step"]) + 1
+    with pytest.raises(ValueError, match="groups"):
+        AdamW(twins[:2]).load_state_dict(saved)
+
+
+@gpu
+@pytest.mark.parametrize("bits", (32, 8))
+def test_captured_steps(bits):
+    """A captured step replayed is the step itself, with the rate read from its tensor."""
+    lr = torch.tensor(0.01, device="cuda")
+    pairs = make((5000, 3, 257), torch.float32, torch.float32, seed=6)
+    twins = [torch.nn.Parameter(p.detach().clone()) for p, _ in pairs]
+    for q, (_, g) in zip(twins, pairs):
+        q.grad = g.clone()
+    a, b = AdamW([p for p, _ in pairs], lr=lr, state_bits=bits), AdamW(twins, lr=0.01, state_bits=bits)
+    a.load_kernels()
+    side = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        a.step()
+    for i in range(4):
+        rate = float(torch.tensor(0.01 * (i + 1), dtype=torch.float32))
+        lr.fill_(rate)
+        b.param_groups[0]["lr"] = rate
+        for (p, g), q in zip(pairs, twins):
+            g.mul_(-0.5)
+            q.grad.copy_(g)
+        graph.replay()
+        b.step()
+    torch.cuda.synchronize()
+    for (p, _), q in zip(pairs, twins):
+        assert torch.equal(p, q) and int(a.state[p]["step"]) == 4
+    for x, y in zip(a.moments(), b.moments()):
+        assert torch.equal(x, y)
+
+
+@gpu
+def test_the_version_counter_moves():
+    p = torch.nn.Parameter(torch.randn(10, device="cuda"))
+    loss = (p * p).sum()
+    p.grad = torch.ones(10, device="cuda")
+    AdamW([p]).step()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
+@gpu
+def test_closures_and_scalers():
+    p = torch.nn.Parameter(torch.ones(4, device="cuda"))
+    opt = AdamW([p], lr=0.1)
+
+    def closure():
+        opt.zero_grad()
+        loss = p.square().sum()
+        loss.backward()
+        return loss
+
+    assert float(opt.step(closure)) == 4.0 and float(p.detach().max()) < 1.0
+    scaler = torch.amp.GradScaler("cuda", init_scale=4.0)
+    opt.zero_grad()
+    scaler.scale((p * math.inf).sum()).backward()
+    before = p.detach().clone()
+    scaler.step(opt)  # gradients that are not finite: no step
+    scaler.update()
+    assert torch.equal(p, before) and int(opt.state[p]["step"]) == 1
+
+
+@gpu
+def test_offsets_past_32_bits():
+    n = (1 << 31) + 777
+    p = torch.nn.Parameter(torch.zeros(n, dtype=torch.bfloat16, device="cuda"))
+    p.grad = torch.zeros(n, dtype=torch.bfloat16, device="cuda")
+    small = torch.nn.Parameter(torch.zeros(777, dtype=torch.bfloat16, device="cuda"))
+    with torch.no_grad():
+        for part in (slice(0, 777), slice(n - 777, n)):
+            p.grad[part] = torch.linspace(-1, 1, 777, device="cuda").to(torch.bfloat16)
+    small.grad = p.grad[:777].clone()
+    for bits in (8,):
+        opt, other = AdamW([p], lr=0.5, state_bits=bits), AdamW([small], lr=0.5, state_bits=bits)
+        opt.step()
+        other.step()
+        assert torch.equal(p[:777], small) and torch.equal(p[n - 777:], small)
+        assert not p[777:n - 777].any()
+        assert torch.equal(opt.state[p]["exp_avg_codes"][:777], other.state[small]["exp_avg_codes"])
+
+
+# ------------------------------------------------------------------------------ refusals
+def test_refusals_on_the_cpu():
+    p = torch.nn.Parameter(torch.ones(5))
+    with pytest.raises(RuntimeError, match="CUDA tensor"):
+        AdamW([p])
+    for kw in (dict(lr=-1.0), dict(lr=math.nan), dict(lr=math.inf), dict(betas=(1.0, 0.9)), dict(betas=(0.9, -0.1)),
+               dict(eps=-1.0), dict(eps=math.nan), dict(weight_decay=-0.1), dict(state_bits=16),
+               dict(lr=torch.tensor(0.1))):
+        with pytest.raises(ValueError):
+            AdamW([p], **kw)
+    with pytest.raises(TypeError, match="float32, bfloat16 or float16"):
+        AdamW([torch.nn.Parameter(torch.ones(5, dtype=torch.float64))])
+    with pytest.raises(ValueError, match="contiguous"):
+        AdamW([torch.nn.Parameter(torch.ones(5, 6).t())])
+
+
+@gpu
+def test_refusals():
+    flat = torch.ones(100, device="cuda")
+    with pytest.raises(ValueError, match="share memory"):
+        AdamW([torch.nn.Parameter(flat[:60]), torch.nn.Parameter(flat[50:])])
+    p, q = (torch.nn.Parameter(torch.ones(8, 4, device="cuda")) for _ in range(2))
+    opt = AdamW([p])
+    with pytest.raises(ValueError):
+        opt.add_param_group({"params": [p]})
+    with pytest.raises(ValueError, match="lr"):
+        opt.add_param_group({"params": [q], "lr": -1.0})
+    assert len(opt.param_groups) == 1 and q not in opt.state
+    p.grad = torch.ones(8, 4, device="cuda").to_sparse()
+    with pytest.raises(RuntimeError, match="dense"):
+        opt.step()
+    p.grad = torch.ones(8, 4, device="cuda")
+    p.data = torch.ones(9, 4, device="cuda")
+    with pytest.raises(RuntimeError, match="size"):
+        opt.step()
+    p.data = torch.ones(4, 8, device="cuda").t()
+    with pytest.raises(RuntimeError, match="layout"):
+        opt.step()
+    p.data = torch.ones(8, 4, device="cuda")
+    opt.param_groups[0]["lr"] = -0.5
+    with pytest.raises(ValueError, match="lr"):
+        opt.step()
+    opt.param_groups[0]["lr"] = 0.5
+    opt.param_groups[0]["params"].append(q)
+    with pytest.raises(RuntimeError, match="changed"):
+        opt.step()
+
+
+def test_c_entries_refuse_bad_parameters():
+    import numpy as np
+
+    from minikg_dev_b200.build import build
+    build()
+    lib = N.load()
+    fake = 4096  # never dereferenced: the host checks come first
+    good_p = dict(lr=0.1, beta1=0.9, beta2=0.99, eps=1e-8, weight_decay=0.0, lr_device=None, param_dtype=0, grad_dtype=0,
+                  state_bits=8, reserved=0)
+    good_s = dict(exp_avg=fake, exp_avg_sq=fake, exp_avg_scale=fake, exp_avg_sq_scale=fake, steps=fake, ticket=fake,
+                  total=512, tensors=2)
+
+    def step(p=(), s=(), params=fake, grads=fake, numel=256, offset=256, index=1):
+        rows = [np.array([x], dtype=np.int64) for x in (params, grads, numel, offset, index)]
+        return lib.mkg_adamw_step(N.AdamwParams(**(good_p | dict(p))), N.AdamwState(**(good_s | dict(s))), 1,
+                                  *(r.ctypes.data for r in rows), None)
+
+    for bad in (dict(p=dict(beta1=1.0)), dict(p=dict(beta2=-0.1)), dict(p=dict(eps=-1.0)), dict(p=dict(weight_decay=-1.0)),
+                dict(p=dict(lr=-1.0)), dict(p=dict(lr=math.nan)), dict(p=dict(param_dtype=3)), dict(p=dict(grad_dtype=-1)),
+                dict(p=dict(state_bits=4)), dict(s=dict(exp_avg=None)), dict(s=dict(exp_avg_scale=None)),
+                dict(s=dict(steps=None)), dict(s=dict(ticket=None)), dict(s=dict(total=500)), dict(s=dict(exp_avg=fake + 4)),
+                dict(params=0), dict(grads=0), dict(numel=257), dict(numel=-1), dict(offset=128), dict(offset=-256),
+                dict(offset=512), dict(index=2), dict(index=-1), dict(params=fake + 2), dict(grads=fake + 1)):
+        assert step(**bad) == 1, bad
+        assert "adamw" in N.last_error()
+    assert lib.mkg_adamw_step(N.AdamwParams(**good_p), N.AdamwState(**good_s), 1, None, None, None, None, None, None) == 1
+    assert lib.mkg_adamw_step(N.AdamwParams(**good_p), N.AdamwState(**good_s), 0, None, None, None, None, None, None) == 0
+    for f in (lib.mkg_adamw_pack, lib.mkg_adamw_unpack):
+        assert f(N.AdamwState(**good_s), None, fake, None) == 1
+        assert f(N.AdamwState(**good_s), fake, fake + 4, None) == 1
+
+
+def test_struct_layouts(tmp_path):
+    import ctypes
+    import subprocess
+    from pathlib import Path
+    root = Path(__file__).resolve().parent.parent
+    for name, cls in (("mkg_adamw_params", N.AdamwParams), ("mkg_adamw_state", N.AdamwState)):
+        fields = [f for f, _ in cls._fields_]
+        src = tmp_path / "layout.c"
+        src.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "minikg_b200.h"\nint main(void) {\n'
+                       + "".join(f'printf("%zu\\n", offsetof({name}, {f}));\n' for f in fields)
+                       + f'printf("%zu\\n", sizeof({name})); return 0; }}\n')
+        subprocess.run(["gcc", "-I", str(root / "include"), str(src), "-o", str(tmp_path / "layout")], check=True)
+        got = [int(v) for v in subprocess.run([str(tmp_path / "layout")], capture_output=True, text=True,
+                                              check=True).stdout.split()]
+        assert got == [getattr(cls, f).offset for f in fields] + [ctypes.sizeof(cls)]
