@@ -613,11 +613,11 @@ enum { MKG_LOGPROB_TOPK_MAX = 32, MKG_LOGPROB_TARGETS_MAX = 1024 };
 typedef struct mkg_logprob_params {
   int64_t rows;
   int64_t width;           /* 1 .. 2^30 */
-  int64_t row_stride;      /* elements from one row of logits to the next */
+  int64_t row_stride;      /* elements from one row of logits to the next; 0: one row stands for all */
   int64_t mask_row_stride; /* bytes from one row of the mask to the next; 0: one row for all */
   int64_t targets;         /* given columns per row, 0 .. MKG_LOGPROB_TARGETS_MAX */
   int64_t topk;            /* alternatives per row, 0 .. MKG_LOGPROB_TOPK_MAX */
-  double tau;              /* > 0 */
+  double tau;              /* 2^-60 .. 2^60 */
   int32_t dtype;           /* MKG_F32 / MKG_BF16 / MKG_F16, of the logits and their gradient */
   int32_t reserved;
 } mkg_logprob_params;
@@ -626,8 +626,8 @@ typedef struct mkg_logprob_params {
  * one that is no candidate gets -inf, one outside [-1, width) gets NaN and sets
  * MKG_DEV_BAD_TARGET), entropy [rows], lse [rows], the topk largest candidates above -inf by
  * logit (ties: the lowest column) as top_ids [rows, topk] / top_logprobs [rows, topk] (-1 / -inf
- * where a row has fewer), and stats [rows, 2] for the backward (the row's largest logit and
- * log2 of the sum of e^{z - its largest}).  A row without a candidate above -inf has lse -inf,
+ * where a row has fewer), and, unless it is NULL, stats [rows, 2] for the backward (the row's largest
+ * logit and log2 of the sum of e^{z - its largest}).  A row without a candidate above -inf has lse -inf,
  * entropy 0 and every log p -inf; a row with NaN or +inf among its candidates has NaN
  * everywhere and no alternatives.  mask may be NULL. */
 size_t mkg_logprob_workspace_bytes(const mkg_logprob_params* p);

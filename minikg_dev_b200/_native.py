@@ -236,8 +236,28 @@ def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream_handle(device: torch.device | None = None) -> int:
+    if _raw_stream is not None and device is not None and device.index is not None:
+        return _raw_stream(device.index)  # the same handle without a Stream object
     return torch.cuda.current_stream(device).cuda_stream
+
+
+class on_device:
+    """``torch.cuda.device(device)``, without its cost where that is the current device already."""
+
+    def __init__(self, device: torch.device):
+        self.guard = None if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
 
 
 def require_cuda(t: torch.Tensor, what: str) -> None:

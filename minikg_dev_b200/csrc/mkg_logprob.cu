@@ -14,7 +14,6 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
-#include <cmath>
 
 #include "mkg_common.cuh"
 #include "mkg_internal.h"
@@ -25,10 +24,13 @@ namespace {
 constexpr float kLn2 = 0.693147180559945309f;
 constexpr float kInf = __builtin_inff();
 constexpr int kTopMax = MKG_LOGPROB_TOPK_MAX;
-constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / kWarp;
-constexpr int kUnroll = 4;           // 16-byte loads in flight per thread
-constexpr int64_t kNarrow = 1024;    // rows up to this width are held by one warp
+// Threads per SM that stream rows.  64 registers each hold a round of loads without spilling; with
+// alternatives and no mask 42 do, and more blocks stream while others order theirs (227 -> 211 us on 64
+// rows of 4,594,485 fp32 logits).
+constexpr int kResident = 1024, kResidentTop = 1536;
+constexpr int kNarrowThreads = 64;   // two rows, a warp each
+constexpr int64_t kNarrow = 2040;    // rows up to this width are held by one warp: 64 values a lane, wherever they start
+constexpr int kCand = 256;           // alternatives collected before they are ordered
 constexpr int64_t kWidthMax = int64_t(1) << 30;
 constexpr unsigned kFull = 0xffffffffu;
 
@@ -69,10 +71,34 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
+// Two fp32 values in one register pair: sm_100 adds, multiplies and fuses them in one instruction.
+using Pair = unsigned long long;
+__device__ __forceinline__ Pair pack2(float a, float b) {
+  Pair r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack2(Pair p, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p)); }
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+  Pair r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+  Pair r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  Pair r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
 // y = (x - m) c with -inf brought to where 2^y is 0 but y stays finite (0 * y must be 0)
 __device__ __forceinline__ float scaled(float x, float m, float c) { return max_nan((x - m) * c, -256.0f); }
 
 template <typename T> constexpr int kVec = 16 / sizeof(T);
+constexpr int kUnroll = 4;  // 16-byte loads in flight per thread
 
 // A row cut into 16-byte slots: slot q holds the columns [q * kVec - lead, + kVec) of the row, so
 // that whole slots start on 16-byte addresses whatever the row's own alignment is.
@@ -89,43 +115,74 @@ template <typename T> struct RowView {
   }
   __device__ __forceinline__ int first(int slot) const { return slot * kVec<T> - lead; }
 
-  // the slot's logits in fp32; columns outside the row and non-candidates as -inf
-  template <bool kMask> __device__ __forceinline__ void load(int slot, float (&v)[kVec<T>]) const {
+  __device__ __forceinline__ bool whole(int slot) const { return first(slot) >= 0 && first(slot) + kVec<T> <= width; }
+
+  // a slot that lies in the row, as it is in memory: its logits and its candidates' bytes
+  struct Raw {
+    uint4 x;
+    uint2 on;
+  };
+  template <bool kMask> __device__ __forceinline__ Raw fetch(int slot) const {
     const int j0 = first(slot);
-    if (j0 >= 0 && j0 + kVec<T> <= width) {
-      const uint4 raw = __ldg(reinterpret_cast<const uint4*>(x + j0));
-      T e[kVec<T>];
-      memcpy(e, &raw, 16);
+    Raw w;
+    w.x = __ldg(reinterpret_cast<const uint4*>(x + j0));
+    if constexpr (kMask) {
+      if (mask_vec) {
+        if constexpr (kVec<T> == 4) w.on.x = __ldg(reinterpret_cast<const uint32_t*>(mask + j0));
+        else w.on = __ldg(reinterpret_cast<const uint2*>(mask + j0));
+      } else {
+        uint8_t on[8];
 #pragma unroll
-      for (int i = 0; i < kVec<T>; ++i) v[i] = to_f32<T>(e[i]);
-      if (kMask) {
-        uint8_t on[kVec<T>];
-        if (mask_vec) {
-          if constexpr (kVec<T> == 4) {
-            const uint32_t b = __ldg(reinterpret_cast<const uint32_t*>(mask + j0));
-            memcpy(on, &b, 4);
-          } else {
-            const uint2 b = __ldg(reinterpret_cast<const uint2*>(mask + j0));
-            memcpy(on, &b, 8);
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < kVec<T>; ++i) on[i] = __ldg(mask + j0 + i);
-        }
-#pragma unroll
-        for (int i = 0; i < kVec<T>; ++i)
-          if (!on[i]) v[i] = -kInf;
+        for (int i = 0; i < kVec<T>; ++i) on[i] = __ldg(mask + j0 + i);
+        memcpy(&w.on, on, 8);
       }
-    } else {
+    }
+    return w;
+  }
+  // in fp32, non-candidates as -inf
+  template <bool kMask> __device__ __forceinline__ void values(const Raw& w, float (&v)[kVec<T>]) const {
+    T e[kVec<T>];
+    memcpy(e, &w.x, 16);
 #pragma unroll
-      for (int i = 0; i < kVec<T>; ++i) {
-        const int j = j0 + i;
-        const bool in = j >= 0 && j < width && (!kMask || __ldg(mask + j) != 0);
-        v[i] = in ? to_f32<T>(x[j]) : -kInf;
-      }
+    for (int i = 0; i < kVec<T>; ++i) v[i] = to_f32<T>(e[i]);
+    if constexpr (kMask) {
+#pragma unroll
+      for (int i = 0; i < kVec<T>; ++i)
+        if (((i < 4 ? w.on.x : w.on.y) >> (8 * (i & 3)) & 255u) == 0) v[i] = -kInf;
+    }
+  }
+  // any slot; columns outside the row as -inf
+  template <bool kMask> __device__ __forceinline__ void load(int slot, float (&v)[kVec<T>]) const {
+    if (whole(slot)) return values<kMask>(fetch<kMask>(slot), v);
+    const int j0 = first(slot);
+#pragma unroll
+    for (int i = 0; i < kVec<T>; ++i) {
+      const int j = j0 + i;
+      const bool in = j >= 0 && j < width && (!kMask || __ldg(mask + j) != 0);
+      v[i] = in ? to_f32<T>(x[j]) : -kInf;
     }
   }
 };
+
+// Hands a thread its slots of [lo, hi), kT apart and in ascending order: whole ones in rounds of up to
+// kUnroll, all of a round's loads before its first use, and those that reach over the row's ends one by
+// one.  many(slot, n, full): n slots from `slot` on; full: n is kUnroll.
+template <typename T, int kT, typename Many, typename One>
+__device__ __forceinline__ void for_slots(const RowView<T>& view, int lo, int hi, int tid, Many many, One one) {
+  int slot = lo + tid;
+  if (slot < hi && !view.whole(slot)) {
+    one(slot);
+    slot += kT;
+  }
+  const int inner = hi == view.slots && hi > lo && !view.whole(hi - 1) ? hi - 1 : hi;
+  for (; slot + (kUnroll - 1) * kT < inner; slot += kUnroll * kT) many(slot, kUnroll, std::true_type());
+  if (slot < inner) {
+    const int n = (inner - slot + kT - 1) / kT;
+    many(slot, n, std::false_type());
+    slot += n * kT;
+  }
+  if (slot < hi) one(slot);
+}
 
 // (value, column) as one word: larger values first, on equal values the lower column; 0 = none
 __device__ __forceinline__ unsigned long long rank_key(float v, uint32_t at) { return pack_value_rank(v + 0.0f, at); }
@@ -176,31 +233,50 @@ __device__ __forceinline__ Moments warp_join(Moments a, float c) {
   return {M, warp_sum(a.s), warp_sum(a.t)};
 }
 
-// The outputs of one row by the threads of a warp or block (`first` of `count`); `best`: the row's
-// largest keys, descending over the lanes of the threads with lane < 32 of the first warp.
+// One given column of a row: what log p needs of it, read before the row is streamed so that the two
+// dependent loads are not waited for at the end.
+struct Target {
+  float x;    // its logit
+  int state;  // 0: padding, 1: a candidate, 2: none, 3: outside the row
+};
+template <typename T>
+__device__ __forceinline__ Target read_target(const Rows& r, const int64_t* targets, int64_t row, int q, const T* x,
+                                              const uint8_t* mask) {
+  Target t{0.0f, 0};
+  if (q >= r.targets) return t;
+  const int64_t id = targets[row * r.targets + q];
+  if (id < -1 || id >= r.width) t.state = 3;
+  else if (id >= 0) {
+    t.state = mask == nullptr || mask[id] != 0 ? 1 : 2;
+    t.x = to_f32<T>(x[id]);
+  }
+  return t;
+}
+
+// The outputs of one row by the threads of a warp or block (`first` of `count`); `mine`: the thread's
+// first target; `best`: the row's largest keys, descending over the lanes of the first warp.
 template <typename T>
 __device__ __forceinline__ void finish_row(const Rows& r, const Outputs& o, int64_t row, const T* x,
-                                           const uint8_t* mask, const int64_t* targets, Moments a,
+                                           const uint8_t* mask, const int64_t* targets, Target mine, Moments a,
                                            unsigned long long best, int first, int count) {
   const bool none = a.m == -kInf && a.s == 0.0f;
   const float log2s = none ? -kInf : a.s == a.s ? log2f(a.s) : a.s;
   if (first == 0) {
     o.lse[row] = none ? -kInf : fmaf(log2s, kLn2, a.m * r.inv_tau) + (a.s - a.s);
     o.entropy[row] = none ? 0.0f : fmaxf(kLn2 * (log2s - a.t / a.s), 0.0f) + (a.s - a.s);
-    o.stats[2 * row] = a.m;
-    o.stats[2 * row + 1] = log2s;
+    if (o.stats) {
+      o.stats[2 * row] = a.m;
+      o.stats[2 * row + 1] = log2s;
+    }
   }
   for (int q = first; q < r.targets; q += count) {
-    const int64_t t = targets[row * r.targets + q];
+    if (q != first) mine = read_target<T>(r, targets, row, q, x, mask);
     float lp = 0.0f;
-    if (t < -1 || t >= r.width) {
+    if (mine.state == 3) {
       raise_flag(o.err, MKG_DEV_BAD_TARGET);
       lp = __int_as_float(0x7fc00000);
-    } else if (t >= 0) {
-      const bool on = mask == nullptr || mask[t] != 0;
-      if (none) lp = -kInf;
-      else if (!on) lp = -kInf + (a.s - a.s);
-      else lp = kLn2 * ((to_f32<T>(x[t]) - a.m) * r.c - log2s);
+    } else if (mine.state != 0) {
+      lp = none ? -kInf : mine.state == 2 ? -kInf + (a.s - a.s) : kLn2 * ((mine.x - a.m) * r.c - log2s);
     }
     o.logprobs[row * r.targets + q] = lp;
   }
@@ -213,46 +289,114 @@ __device__ __forceinline__ void finish_row(const Rows& r, const Outputs& o, int6
   }
 }
 
-// ---------------------------------------------------------------- rows of up to 1024 columns: a warp each
-template <typename T, bool kMask, int kPer>
-__global__ void __launch_bounds__(kThreads) logprob_narrow_kernel(Rows r, const T* __restrict__ logits,
-                                                                  const uint8_t* __restrict__ masks,
-                                                                  const int64_t* __restrict__ targets, Outputs o) {
-  const int lane = threadIdx.x & 31;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
+// ---------------------------------------------------------------- the largest keys of a warp or block
+// The topk-th largest of one key per thread of the block, 0 if there are fewer; sh: a key per thread.
+template <int kWarps>
+__device__ __forceinline__ unsigned long long floor_of(unsigned long long mine, int topk, unsigned long long* sh) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  unsigned long long v = sort_ascending(mine, lane);
+  unsigned long long best = __shfl_sync(kFull, v, 31 - lane);
+#pragma unroll
+  for (int half = kWarps / 2; half > 0; half >>= 1) {  // the upper half of the warps hands its 32 to the lower
+    if (warp >= half && warp < 2 * half) sh[warp * kWarp + (31 - lane)] = best;
+    __syncthreads();
+    if (warp < half) best = merge_best(best, sh[(warp + half) * kWarp + lane], lane);
+    __syncthreads();
+  }
+  if (threadIdx.x == topk - 1) sh[0] = best;
+  __syncthreads();
+  return sh[0];
+}
+// The warp's part of a list of keys in shared memory, merged into `best`.
+__device__ __forceinline__ unsigned long long merge_list(unsigned long long best, const unsigned long long* list, int n,
+                                                         int lane) {
+  for (int i = 0; i < n; i += kWarp)
+    best = merge_best(best, sort_ascending(i + lane < n ? list[i + lane] : 0, lane), lane);
+  return best;
+}
+
+// ---------------------------------------------------------------- narrow rows: a warp each
+template <typename T, bool kMask, int kSlots>
+__global__ void __launch_bounds__(kNarrowThreads) logprob_narrow_kernel(Rows r, const T* __restrict__ logits,
+                                                                        const uint8_t* __restrict__ masks,
+                                                                        const int64_t* __restrict__ targets, Outputs o) {
+  __shared__ unsigned long long sh_cand[kNarrowThreads / kWarp][2 * kWarp];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kNarrowThreads / kWarp) + warp;
   if (row >= r.rows) return;
   const T* x = logits + row * r.stride;
   const uint8_t* mask = kMask ? masks + row * r.mask_stride : nullptr;
-  float v[kPer];
-  Moments a{-kInf, 0.0f, 0.0f};
+  const RowView<T> view(x, mask, r.width);
+  const Target target = read_target<T>(r, targets, row, lane, x, mask);
+  float v[kSlots][kVec<T>];
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const int j = i * kWarp + lane;
-    v[i] = j < r.width && (!kMask || mask[j] != 0) ? to_f32<T>(x[j]) : -kInf;
-    a.m = fmaxf(a.m, v[i]);
+  for (int q = 0; q < kSlots; ++q) {
+    const int slot = q * kWarp + lane;
+    if (slot < view.slots) {
+      view.template load<kMask>(slot, v[q]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kVec<T>; ++i) v[q][i] = -kInf;
+    }
   }
+  Moments a{-kInf, 0.0f, 0.0f};
+  int at = 0;  // the column where the lane first met its largest
+#pragma unroll
+  for (int q = 0; q < kSlots; ++q)
+#pragma unroll
+    for (int i = 0; i < kVec<T>; ++i)
+      if (v[q][i] > a.m) {
+        a.m = v[q][i];
+        at = view.first(q * kWarp + lane) + i;
+      }
+  const unsigned long long mine = a.m > -kInf ? rank_key(a.m, static_cast<uint32_t>(at)) : 0;
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) a.m = fmaxf(a.m, __shfl_xor_sync(kFull, a.m, off));
   const float from = a.m == -kInf ? 0.0f : a.m;
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const float y = scaled(v[i], from, r.c);
-    const float e = ex2(y);
-    a.s += e;
-    a.t = fmaf(e, y, a.t);
-  }
+  for (int q = 0; q < kSlots; ++q)
+#pragma unroll
+    for (int i = 0; i < kVec<T>; ++i) {
+      const float y = scaled(v[q][i], from, r.c);
+      const float e = ex2(y);
+      a.s += e;
+      a.t = fmaf(e, y, a.t);
+    }
   a.s = warp_sum(a.s);
   a.t = warp_sum(a.t);
   unsigned long long best = 0;
   if (r.topk > 0) {
+    // elements below the topk-th largest of the lanes' maxima have topk better ones
+    const unsigned long long sorted = sort_ascending(mine, lane);
+    const unsigned long long floor = __shfl_sync(kFull, sorted, 32 - r.topk);
+    const float least = floor ? packed_value(floor) : -kInf;
+    const int least_at = floor ? static_cast<int>(packed_rank(floor)) : 0x7fffffff;
+    unsigned long long* cand = sh_cand[warp];
+    int n = 0;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      unsigned long long k = v[i] > -kInf ? rank_key(v[i], i * kWarp + lane) : 0;
-      const unsigned long long worst = __shfl_sync(kFull, best, r.topk - 1);
-      if (__any_sync(kFull, k > worst)) best = merge_best(best, sort_ascending(k, lane), lane);
+    for (int q = 0; q < kSlots; ++q)
+#pragma unroll
+      for (int i = 0; i < kVec<T>; ++i) {
+        const int j = view.first(q * kWarp + lane) + i;
+        const bool in = v[q][i] > least || (v[q][i] == least && v[q][i] > -kInf && j <= least_at);
+        const unsigned who = __ballot_sync(kFull, in);
+        const int to = n + __popc(who & ((1u << lane) - 1));
+        if (in && to < 2 * kWarp) cand[to] = rank_key(v[q][i], static_cast<uint32_t>(j));
+        n += __popc(who);
+      }
+    __syncwarp();
+    if (n <= 2 * kWarp) {
+      best = merge_list(0, cand, n, lane);
+    } else {  // a few lanes hold many of the largest: merge the row as it comes
+      for (int j = lane; j < ((r.width + kWarp - 1) & -kWarp); j += kWarp) {
+        const float w = j < r.width && (!kMask || mask[j] != 0) ? to_f32<T>(x[j]) : -kInf;
+        const unsigned long long k = w > -kInf ? rank_key(w, static_cast<uint32_t>(j)) : 0;
+        if (__any_sync(kFull, k > __shfl_sync(kFull, best, r.topk - 1)))
+          best = merge_best(best, sort_ascending(k, lane), lane);
+      }
     }
   }
-  finish_row<T>(r, o, row, x, mask, targets, a, best, lane, kWarp);
+  finish_row<T>(r, o, row, x, mask, targets, target, a, best, lane, kWarp);
 }
 
 // ---------------------------------------------------------------- wider rows: blocks, joined if several
@@ -260,16 +404,67 @@ struct Partial {
   float m, s, t, pad;
 };
 
-template <typename T, bool kMask, bool kTop>
-__global__ void __launch_bounds__(kThreads) logprob_wide_kernel(Rows r, const T* __restrict__ logits,
-                                                                const uint8_t* __restrict__ masks,
-                                                                const int64_t* __restrict__ targets, Outputs o,
-                                                                int splits, int slots_per_split,
-                                                                Partial* __restrict__ partials,
-                                                                unsigned long long* __restrict__ keys) {
-  __shared__ float sh_m[kWarps], sh_s[kWarps], sh_t[kWarps];
-  __shared__ unsigned long long sh_key[kThreads];
-  __shared__ int sh_winner[kWarp];
+// Joins the warps' (m, s, t) of a block; every thread gets the result.
+template <int kWarps> __device__ __forceinline__ Moments block_join(Moments a, float c, Moments* sh) {
+  const int lane = threadIdx.x & 31;
+  a = warp_join(a, c);
+  if (lane == 0) sh[threadIdx.x >> 5] = a;
+  __syncthreads();
+  return warp_join(lane < kWarps ? sh[lane] : Moments{-kInf, 0.0f, 0.0f}, c);
+}
+
+// A thread's share of a row while it streams: the largest element and where it was first met, and the
+// sums seen from `ref`.  ref follows m only when 2^y would pass 2^kMargin: in a warp some lane meets a
+// new maximum in most rounds, and rescaling each time took half of the loop's instructions.
+constexpr float kMargin = 8.0f;
+struct Stream {
+  float m, ref, limit;  // limit = ref + kMargin / c
+  int at;
+  Pair s, t;
+};
+template <typename T> __device__ __forceinline__ void consume(const float (&v)[kVec<T>], int slot, float c, Stream& a) {
+  float big = v[0];
+#pragma unroll
+  for (int i = 1; i < kVec<T>; ++i) big = fmaxf(big, v[i]);
+  if (big > a.m) {
+    a.m = big;
+    a.at = slot;
+  }
+  if (big > a.limit) {
+    float s0, s1, t0, t1;
+    unpack2(a.s, s0, s1);
+    unpack2(a.t, t0, t1);
+    Moments lo{a.ref, s0, t0}, hi{a.ref, s1, t1};
+    shift_to(lo, big, c);
+    shift_to(hi, big, c);
+    a.s = pack2(lo.s, hi.s);
+    a.t = pack2(lo.t, hi.t);
+    a.ref = big;
+    a.limit = big + kMargin / c;
+  }
+  const float from = a.ref == -kInf ? 0.0f : a.ref;
+  const Pair from2 = pack2(-from, -from), c2 = pack2(c, c);
+#pragma unroll
+  for (int i = 0; i < kVec<T>; i += 2) {
+    float y0, y1;
+    unpack2(mul2(add2(pack2(v[i], v[i + 1]), from2), c2), y0, y1);
+    y0 = max_nan(y0, -256.0f);
+    y1 = max_nan(y1, -256.0f);
+    const Pair e = pack2(ex2(y0), ex2(y1));
+    a.s = add2(a.s, e);
+    a.t = fma2(e, pack2(y0, y1), a.t);
+  }
+}
+
+template <typename T, bool kMask, bool kTop, int kT>
+__global__ void __launch_bounds__(kT, (kTop && !kMask ? kResidentTop : kResident) / kT)
+    logprob_wide_kernel(Rows r, const T* __restrict__ logits, const uint8_t* __restrict__ masks,
+                        const int64_t* __restrict__ targets, Outputs o, int splits, int slots_per_split,
+                        Partial* __restrict__ partials, unsigned long long* __restrict__ keys) {
+  constexpr int kWarps = kT / kWarp;
+  __shared__ Moments sh_m[kWarps];
+  __shared__ unsigned long long sh_key[kTop ? kT : 1], sh_cand[kTop ? kCand : 1];
+  __shared__ int sh_winner[kTopMax], sh_winners, sh_n;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t row = blockIdx.x / splits;
   const int split = static_cast<int>(blockIdx.x % splits);
@@ -278,80 +473,55 @@ __global__ void __launch_bounds__(kThreads) logprob_wide_kernel(Rows r, const T*
   const RowView<T> view(x, mask, r.width);
   const int lo = split * slots_per_split;
   const int hi = min(lo + slots_per_split, view.slots);
+  if (kTop && tid == 0) sh_n = sh_winners = 0;
+  Target target{0.0f, 0};
+  if (splits > 1) cudaTriggerProgrammaticLaunchCompletion();  // the joining kernel may come and wait
+  else target = read_target<T>(r, targets, row, tid, x, mask);
 
-  Moments a{-kInf, 0.0f, 0.0f};
-  int at = 0;  // the slot where the thread first met a.m
-  for (int base = lo + tid; base < hi; base += kThreads * kUnroll) {
-    float v[kUnroll][kVec<T>];
+  Stream own{-kInf, -kInf, -kInf, 0, 0, 0};
+  for_slots<T, kT>(
+      view, lo, hi, tid,
+      [&](int slot, int n, auto full) {
+        typename RowView<T>::Raw raw[kUnroll];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int slot = base + u * kThreads;
-      if (slot < hi) {
-        view.template load<kMask>(slot, v[u]);
-      } else {
+        for (int u = 0; u < kUnroll; ++u)
+          if (full || u < n) raw[u] = view.template fetch<kMask>(slot + u * kT);
 #pragma unroll
-        for (int i = 0; i < kVec<T>; ++i) v[u][i] = -kInf;
-      }
-    }
-    float M = a.m;
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      float big = v[u][0];
-#pragma unroll
-      for (int i = 1; i < kVec<T>; ++i) big = fmaxf(big, v[u][i]);
-      if (big > M) {
-        M = big;
-        at = base + u * kThreads;
-      }
-    }
-    if (M > a.m) {
-      shift_to(a, M, r.c);
-      a.m = M;
-    }
-    const float from = M == -kInf ? 0.0f : M;
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u)
-#pragma unroll
-      for (int i = 0; i < kVec<T>; ++i) {
-        const float y = scaled(v[u][i], from, r.c);
-        const float e = ex2(y);
-        a.s += e;
-        a.t = fmaf(e, y, a.t);
-      }
-  }
-  const unsigned long long mine = a.m > -kInf ? rank_key(a.m, static_cast<uint32_t>(at)) : 0;
+        for (int u = 0; u < kUnroll; ++u) {
+          if (!full && u >= n) break;
+          float v[kVec<T>];
+          view.template values<kMask>(raw[u], v);
+          consume<T>(v, slot + u * kT, r.c, own);
+        }
+      },
+      [&](int slot) {
+        float v[kVec<T>];
+        view.template load<kMask>(slot, v);
+        consume<T>(v, slot, r.c, own);
+      });
+  float s0, s1, t0, t1;
+  unpack2(own.s, s0, s1);
+  unpack2(own.t, t0, t1);
+  Moments a{own.ref, s0 + s1, t0 + t1};
+  shift_to(a, own.m, r.c);
+  a.m = own.m;
+  const unsigned long long mine = a.m > -kInf ? rank_key(a.m, static_cast<uint32_t>(own.at)) : 0;
+  const Moments all = block_join<kWarps>(a, r.c, sh_m);
 
-  Moments all = warp_join(a, r.c);
-  if (lane == 0) {
-    sh_m[warp] = all.m;
-    sh_s[warp] = all.s;
-    sh_t[warp] = all.t;
-  }
   unsigned long long best = 0;
-  if (kTop) sh_key[tid] = sort_ascending(mine, lane);
-  __syncthreads();
-  {
-    Moments b = lane < kWarps ? Moments{sh_m[lane], sh_s[lane], sh_t[lane]} : Moments{-kInf, 0.0f, 0.0f};
-    all = warp_join(b, r.c);
-  }
   if (kTop) {
-    // the topk best threads, by (largest element, where it was first met)
-    unsigned long long top = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) top = merge_best(top, sh_key[w * kWarp + lane], lane);
-    // a slot's position names its thread: slots are dealt out in turn
-    if (warp == 0)
-      sh_winner[lane] = top != 0 && lane < r.topk
-                            ? static_cast<int>((packed_rank(top) - static_cast<uint32_t>(lo)) % kThreads) : -1;
-    const unsigned long long floor_key = __shfl_sync(kFull, top, r.topk - 1);
-    const float least = floor_key != 0 ? packed_value(floor_key) : -kInf;
-    const uint32_t least_slot = floor_key != 0 ? packed_rank(floor_key) : 0xffffffffu;
+    // threads whose largest element is among the topk largest such have their elements read again
+    const unsigned long long floor = floor_of<kWarps>(mine, r.topk, sh_key);
+    const float least = floor ? packed_value(floor) : -kInf;
+    const uint32_t least_slot = floor ? packed_rank(floor) : 0xffffffffu;
+    if (mine != 0 && mine >= floor) sh_winner[atomicAdd(&sh_winners, 1)] = tid;  // at most topk: keys differ
     __syncthreads();
-    for (int w = warp; w < r.topk; w += kWarps) {
-      const int who = sh_winner[w];
-      if (who < 0) continue;
-      for (int base = lo + who; base < hi; base += kThreads * kWarp) {
-        const int slot = base + lane * kThreads;
+    const int per = (hi - lo + kT - 1) / kT;  // slots of a thread
+    // `use` gets the lanes' keys of one element each, 0 for those that cannot be among the topk
+    auto again = [&](auto use) {
+      const int pairs = sh_winners * per;
+      for (int q = tid; q < ((pairs + kWarp - 1) & -kWarp); q += kT) {
+        const int slot = q < pairs ? lo + sh_winner[q / per] + q % per * kT : hi;
         float v[kVec<T>];
         if (slot < hi) {
           view.template load<kMask>(slot, v);
@@ -362,21 +532,31 @@ __global__ void __launch_bounds__(kThreads) logprob_wide_kernel(Rows r, const T*
 #pragma unroll
         for (int i = 0; i < kVec<T>; ++i) {
           const bool in = v[i] > least || (v[i] == least && v[i] > -kInf && static_cast<uint32_t>(slot) <= least_slot);
-          const unsigned long long k = in ? rank_key(v[i], static_cast<uint32_t>(view.first(slot) + i)) : 0;
-          const unsigned long long worst = __shfl_sync(kFull, best, r.topk - 1);
-          if (__any_sync(kFull, k > worst)) best = merge_best(best, sort_ascending(k, lane), lane);
+          use(in ? rank_key(v[i], static_cast<uint32_t>(view.first(slot) + i)) : 0);
         }
       }
+    };
+    again([&](unsigned long long k) {
+      if (k != 0) {
+        const int n = atomicAdd(&sh_n, 1);  // any order: they are sorted below
+        if (n < kCand) sh_cand[n] = k;
+      }
+    });
+    __syncthreads();
+    if (sh_n <= kCand) {
+      if (warp == 0) best = merge_list(0, sh_cand, sh_n, lane);
+    } else {  // few threads hold many of the largest: merge as they come
+      again([&](unsigned long long k) {
+        if (__any_sync(kFull, k > __shfl_sync(kFull, best, r.topk - 1)))
+          best = merge_best(best, sort_ascending(k, lane), lane);
+      });
+      sh_key[tid] = best;
+      __syncthreads();
+      if (warp == 0) best = merge_list(0, sh_key, kT, lane);
     }
-    __syncthreads();
-    sh_key[warp * kWarp + (31 - lane)] = best;  // ascending
-    __syncthreads();
-    best = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) best = merge_best(best, sh_key[w * kWarp + lane], lane);
   }
   if (splits == 1) {
-    finish_row<T>(r, o, row, x, mask, targets, all, best, tid, kThreads);
+    finish_row<T>(r, o, row, x, mask, targets, target, all, best, tid, kT);
   } else {
     const int64_t at_split = row * splits + split;
     if (tid == 0) partials[at_split] = {all.m, all.s, all.t, 0.0f};
@@ -384,48 +564,71 @@ __global__ void __launch_bounds__(kThreads) logprob_wide_kernel(Rows r, const T*
   }
 }
 
-// One block per row joins its splits in their order.
+// One block per row joins its splits, always in the same order.
+constexpr int kJoinThreads = 256;
 template <typename T, bool kMask>
-__global__ void __launch_bounds__(kThreads) logprob_join_kernel(Rows r, const T* __restrict__ logits,
-                                                                const uint8_t* __restrict__ masks,
-                                                                const int64_t* __restrict__ targets, Outputs o,
-                                                                int splits, const Partial* __restrict__ partials,
-                                                                const unsigned long long* __restrict__ keys) {
-  __shared__ float sh_m[kWarps], sh_s[kWarps], sh_t[kWarps];
-  __shared__ unsigned long long sh_key[kThreads];
+__global__ void __launch_bounds__(kJoinThreads) logprob_join_kernel(Rows r, const T* __restrict__ logits,
+                                                                    const uint8_t* __restrict__ masks,
+                                                                    const int64_t* __restrict__ targets, Outputs o,
+                                                                    int splits, const Partial* __restrict__ partials,
+                                                                    const unsigned long long* __restrict__ keys) {
+  constexpr int kWarps = kJoinThreads / kWarp;
+  __shared__ Moments sh_m[kWarps];
+  __shared__ unsigned long long sh_key[kJoinThreads], sh_cand[kCand];
+  __shared__ int sh_n;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t row = blockIdx.x;
-  Moments a{-kInf, 0.0f, 0.0f};
-  for (int i = tid; i < splits; i += kThreads) {
-    const Partial p = partials[row * splits + i];
-    Moments b{p.m, p.s, p.t};
-    const float M = fmaxf(a.m, b.m);
-    shift_to(a, M, r.c);
-    shift_to(b, M, r.c);
-    a = {M, a.s + b.s, a.t + b.t};
-  }
-  Moments all = warp_join(a, r.c);
-  if (lane == 0) {
-    sh_m[warp] = all.m;
-    sh_s[warp] = all.s;
-    sh_t[warp] = all.t;
-  }
-  unsigned long long best = 0;
-  const int n = splits * r.topk;  // 0: nothing to merge
-  for (int i = warp * kWarp; i < n; i += kThreads) {
-    const unsigned long long k = i + lane < n ? keys[row * n + i + lane] : 0;
-    const unsigned long long worst = __shfl_sync(kFull, best, r.topk - 1);
-    if (__any_sync(kFull, k > worst)) best = merge_best(best, sort_ascending(k, lane), lane);
-  }
-  sh_key[warp * kWarp + (31 - lane)] = best;
-  __syncthreads();
-  Moments b = lane < kWarps ? Moments{sh_m[lane], sh_s[lane], sh_t[lane]} : Moments{-kInf, 0.0f, 0.0f};
-  all = warp_join(b, r.c);
-  best = 0;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) best = merge_best(best, sh_key[w * kWarp + lane], lane);
   const T* x = logits + row * r.stride;
-  finish_row<T>(r, o, row, x, kMask ? masks + row * r.mask_stride : nullptr, targets, all, best, tid, kThreads);
+  const uint8_t* mask = kMask ? masks + row * r.mask_stride : nullptr;
+  const Target target = read_target<T>(r, targets, row, tid, x, mask);
+  if (tid == 0) sh_n = 0;
+  Moments a{-kInf, 0.0f, 0.0f};
+  unsigned long long mine = 0, best = 0;
+  const unsigned long long* list = keys + row * splits * r.topk;
+  cudaGridDependencySynchronize();  // launched while the blocks before it still run
+  constexpr int kAhead = 4;
+  for (int i = tid; i < splits; i += kJoinThreads * kAhead) {
+    Partial p[kAhead];
+    unsigned long long k[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int j = i + u * kJoinThreads;
+      p[u] = j < splits ? partials[row * splits + j] : Partial{-kInf, 0.0f, 0.0f, 0.0f};
+      k[u] = j < splits && r.topk > 0 ? list[static_cast<int64_t>(j) * r.topk] : 0;  // a split's keys descend
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      Moments b{p[u].m, p[u].s, p[u].t};
+      const float M = fmaxf(a.m, b.m);
+      shift_to(a, M, r.c);
+      shift_to(b, M, r.c);
+      a = {M, a.s + b.s, a.t + b.t};
+      mine = max(mine, k[u]);
+    }
+  }
+  const Moments all = block_join<kWarps>(a, r.c, sh_m);
+  if (r.topk > 0) {
+    const unsigned long long floor = max(floor_of<kWarps>(mine, r.topk, sh_key), 1ull);
+    for (int i = tid; i < splits; i += kJoinThreads)
+      for (int q = 0; q < r.topk; ++q) {
+        const unsigned long long k = list[static_cast<int64_t>(i) * r.topk + q];
+        if (k < floor) break;
+        const int n = atomicAdd(&sh_n, 1);
+        if (n < kCand) sh_cand[n] = k;
+      }
+    __syncthreads();
+    if (sh_n <= kCand) {
+      if (warp == 0) best = merge_list(0, sh_cand, sh_n, lane);
+    } else if (warp == 0) {
+      const int64_t n = static_cast<int64_t>(splits) * r.topk;
+      for (int64_t i = 0; i < n; i += kWarp) {
+        const unsigned long long k = i + lane < n ? list[i + lane] : 0;
+        if (__any_sync(kFull, k > __shfl_sync(kFull, best, r.topk - 1)))
+          best = merge_best(best, sort_ascending(k, lane), lane);
+      }
+    }
+  }
+  finish_row<T>(r, o, row, x, mask, targets, target, all, best, tid, kJoinThreads);
 }
 
 // ---------------------------------------------------------------- gradient
@@ -479,11 +682,123 @@ __device__ __forceinline__ float share(const RowGrad& g, float x, float c) {
   return ex2(y) * fmaf(g.b, y, g.a);
 }
 
+// The named columns [j_lo, j_hi) once more, with their own gradients added before the one rounding:
+// the first to name a column writes it, with all that is named there added in order.
+template <typename T, bool kMask, typename Id, typename G>
+__device__ __forceinline__ void add_named(const Rows& r, const RowGrad& g, const T* x, const uint8_t* mask, T* grad,
+                                          int j_lo, int j_hi, int first, int count, Id id_of, G grad_of) {
+  const int n = r.targets + r.topk;
+  for (int q = first; q < n; q += count) {
+    const int id = id_of(q);
+    if (id < j_lo || id >= j_hi || id < 0 || (kMask && mask[id] == 0)) continue;
+    float add = 0.0f;
+    bool again = false;
+    for (int k = 0; k < n; ++k)
+      if (id_of(k) == id) {
+        again |= k < q;
+        add += grad_of(k);
+      }
+    if (!again) grad[id] = from_f32<T>(fmaf(add, r.inv_tau, share(g, to_f32<T>(x[id]), r.c)));
+  }
+}
+
+// The gradient of a slot's columns.
 template <typename T, bool kMask>
-__global__ void __launch_bounds__(kThreads) logprob_backward_kernel(Rows r, const T* __restrict__ logits,
-                                                                    const uint8_t* __restrict__ masks, Upstream u,
-                                                                    T* __restrict__ grads, int splits,
-                                                                    int slots_per_split) {
+__device__ __forceinline__ void slot_grad(const RowGrad& g, float c, const float (&v)[kVec<T>], T (&out)[kVec<T>]) {
+  const Pair m2 = pack2(-g.m, -g.m), c2 = pack2(c, c), l2 = pack2(-g.log2s, -g.log2s);
+  const Pair a2 = pack2(g.a, g.a), b2 = pack2(g.b, g.b);
+#pragma unroll
+  for (int i = 0; i < kVec<T>; i += 2) {
+    float y0, y1, d0, d1;
+    unpack2(fma2(add2(pack2(v[i], v[i + 1]), m2), c2, l2), y0, y1);
+    y0 = max_nan(y0, -256.0f);
+    y1 = max_nan(y1, -256.0f);
+    unpack2(mul2(pack2(ex2(y0), ex2(y1)), fma2(b2, pack2(y0, y1), a2)), d0, d1);
+    // a non-candidate reads as -inf: its share is 0 unless the row itself is NaN
+    out[i] = from_f32<T>(g.none || (kMask && v[i] == -kInf) ? 0.0f : d0);
+    out[i + 1] = from_f32<T>(g.none || (kMask && v[i + 1] == -kInf) ? 0.0f : d1);
+  }
+}
+
+// The gradient of a thread's slots of [lo, hi), kT apart.
+template <typename T, bool kMask, int kT>
+__device__ __forceinline__ void slots_grad(const RowView<T>& view, int lo, int hi, int tid, const RowGrad& g, float c,
+                                           T* grad) {
+  const bool store_vec = (reinterpret_cast<uintptr_t>(grad) - view.lead * sizeof(T)) % 16 == 0;
+  auto store = [&](int slot, const T(&out)[kVec<T>], bool whole) {
+    const int j0 = view.first(slot);
+    if (store_vec && whole) {
+      uint4 raw;
+      memcpy(&raw, out, 16);
+      __stcs(reinterpret_cast<uint4*>(grad + j0), raw);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kVec<T>; ++i)
+        if (j0 + i >= 0 && j0 + i < view.width) grad[j0 + i] = out[i];
+    }
+  };
+  for_slots<T, kT>(
+      view, lo, hi, tid,
+      [&](int slot, int n, auto full) {
+        typename RowView<T>::Raw raw[kUnroll];
+#pragma unroll
+        for (int w = 0; w < kUnroll; ++w)
+          if (full || w < n) raw[w] = view.template fetch<kMask>(slot + w * kT);
+#pragma unroll
+        for (int w = 0; w < kUnroll; ++w) {
+          if (!full && w >= n) break;
+          float v[kVec<T>];
+          T out[kVec<T>];
+          view.template values<kMask>(raw[w], v);
+          slot_grad<T, kMask>(g, c, v, out);
+          store(slot + w * kT, out, true);
+        }
+      },
+      [&](int slot) {
+        float v[kVec<T>];
+        T out[kVec<T>];
+        view.template load<kMask>(slot, v);
+        slot_grad<T, kMask>(g, c, v, out);
+        store(slot, out, false);
+      });
+}
+
+// A warp per row, for narrow rows with few named columns.
+constexpr int kNamedNarrow = 64;
+template <typename T, bool kMask>
+__global__ void __launch_bounds__(kNarrowThreads) logprob_backward_narrow_kernel(Rows r, const T* __restrict__ logits,
+                                                                                 const uint8_t* __restrict__ masks,
+                                                                                 Upstream u, T* __restrict__ grads) {
+  __shared__ int sh_id[kNarrowThreads / kWarp][kNamedNarrow];
+  __shared__ float sh_g[kNarrowThreads / kWarp][kNamedNarrow];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kNarrowThreads / kWarp) + warp;
+  if (row >= r.rows) return;
+  const T* x = logits + row * r.stride;
+  const uint8_t* mask = kMask ? masks + row * r.mask_stride : nullptr;
+  T* grad = grads + row * r.width;
+  float sum = 0.0f;
+  for (int q = lane; q < r.targets + r.topk; q += kWarp) {
+    int64_t id;
+    const float g = named(r, u, row, q, id);
+    sh_id[warp][q] = static_cast<int>(id);
+    sh_g[warp][q] = g;
+    sum += g;
+  }
+  const RowGrad g = row_grad(r, u, row, warp_sum(sum));
+  const RowView<T> view(x, mask, r.width);
+  slots_grad<T, kMask, kWarp>(view, 0, view.slots, lane, g, r.c, grad);
+  __syncwarp();
+  if (!g.none)
+    add_named<T, kMask>(r, g, x, mask, grad, 0, r.width, lane, kWarp, [&](int q) { return sh_id[warp][q]; },
+                        [&](int q) { return sh_g[warp][q]; });
+}
+
+template <typename T, bool kMask, int kT>
+__global__ void __launch_bounds__(kT, kResident / kT)
+    logprob_backward_kernel(Rows r, const T* __restrict__ logits, const uint8_t* __restrict__ masks, Upstream u,
+                            T* __restrict__ grads, int splits, int slots_per_split) {
+  constexpr int kWarps = kT / kWarp;
   extern __shared__ int sh_id[];  // [named], then their gradients
   __shared__ float sh_sum[kWarps];
   const int named_n = r.targets + r.topk;
@@ -497,7 +812,7 @@ __global__ void __launch_bounds__(kThreads) logprob_backward_kernel(Rows r, cons
   const RowView<T> view(x, mask, r.width);
 
   float sum = 0.0f;
-  for (int q = tid; q < named_n; q += kThreads) {
+  for (int q = tid; q < named_n; q += kT) {
     int64_t id;
     const float g = named(r, u, row, q, id);
     sh_id[q] = static_cast<int>(id);
@@ -514,44 +829,11 @@ __global__ void __launch_bounds__(kThreads) logprob_backward_kernel(Rows r, cons
 
   const int lo = split * slots_per_split;
   const int hi = min(lo + slots_per_split, view.slots);
-  const bool store_vec = (reinterpret_cast<uintptr_t>(grad) - view.lead * sizeof(T)) % 16 == 0;
-  for (int slot = lo + tid; slot < hi; slot += kThreads) {
-    float v[kVec<T>];
-    view.template load<kMask>(slot, v);
-    const int j0 = view.first(slot);
-    T out[kVec<T>];
-#pragma unroll
-    for (int i = 0; i < kVec<T>; ++i) {
-      // a non-candidate reads as -inf: its share is 0 unless the row itself is NaN
-      const bool off = g.none || (kMask && v[i] == -kInf);
-      out[i] = from_f32<T>(off ? 0.0f : share(g, v[i], r.c));
-    }
-    if (store_vec && j0 >= 0 && j0 + kVec<T> <= r.width) {
-      uint4 raw;
-      memcpy(&raw, out, 16);
-      *reinterpret_cast<uint4*>(grad + j0) = raw;
-    } else {
-#pragma unroll
-      for (int i = 0; i < kVec<T>; ++i)
-        if (j0 + i >= 0 && j0 + i < r.width) grad[j0 + i] = out[i];
-    }
-  }
-  if (named_n == 0 || g.none) return;
+  slots_grad<T, kMask, kT>(view, lo, hi, tid, g, r.c, grad);
+  if (named_n == 0 || g.none || lo >= hi) return;
   __syncthreads();
-  // the named columns of this block again, with their own gradients added before the one rounding
-  const int j_lo = view.first(lo), j_hi = view.first(hi);
-  for (int q = tid; q < named_n; q += kThreads) {
-    const int id = sh_id[q];
-    if (id < 0 || id < j_lo || id >= j_hi || (kMask && mask[id] == 0)) continue;
-    float add = 0.0f;
-    bool again = false;
-    for (int k = 0; k < named_n; ++k)
-      if (sh_id[k] == id) {
-        again |= k < q;  // the first to name the column writes it
-        add += sh_g[k];
-      }
-    if (!again) grad[id] = from_f32<T>(fmaf(add, r.inv_tau, share(g, to_f32<T>(x[id]), r.c)));
-  }
+  add_named<T, kMask>(r, g, x, mask, grad, view.first(lo), view.first(hi), tid, kT, [&](int q) { return sh_id[q]; },
+                      [&](int q) { return sh_g[q]; });
 }
 
 int check_params(const mkg_logprob_params* p, Rows* r) {
@@ -563,31 +845,47 @@ int check_params(const mkg_logprob_params* p, Rows* r) {
               (long long)p->targets, (int)MKG_LOGPROB_TARGETS_MAX);
   MKG_REQUIRE(p->topk >= 0 && p->topk <= kTopMax, "logprob: topk %lld outside [0, %d]", (long long)p->topk, kTopMax);
   MKG_REQUIRE(p->dtype >= MKG_F32 && p->dtype <= MKG_F16, "logprob: unknown element type %d", p->dtype);
-  MKG_REQUIRE(p->tau > 0.0 && std::isfinite(p->tau), "logprob: tau must be positive and finite");
+  MKG_REQUIRE(p->tau >= 0x1p-60 && p->tau <= 0x1p60, "logprob: tau %g outside [2^-60, 2^60]", p->tau);
   MKG_REQUIRE(p->row_stride >= 0 && p->mask_row_stride >= 0, "logprob: negative row stride");
   *r = Rows{p->rows, p->row_stride, p->mask_row_stride, (int)p->width, (int)p->targets, (int)p->topk,
             (float)(1.4426950408889634 / p->tau), (float)(1.0 / p->tau)};
   return MKG_OK;
 }
 
+// How rows are dealt to blocks: `splits` pieces of `slots` 16-byte slots per row.
 struct Cut {
-  int splits, slots;
+  int splits, slots, threads;
 };
-// Blocks per row: enough that all rows together fill the SMs several times over, each with at
-// least `least` rounds of loads.
-Cut cut_rows(const mkg_logprob_params* p, int per_sm, int least) {
+int64_t most_slots(const mkg_logprob_params* p) {  // of a row, wherever it starts
   const int vec = p->dtype == MKG_F32 ? 4 : 8;
-  const int64_t slots = (p->width + 2 * vec - 2) / vec;  // the most a row can have
-  const int64_t round = (int64_t)kThreads * kUnroll;
-  const int64_t want = ((int64_t)persistent_blocks(per_sm) + p->rows - 1) / std::max<int64_t>(p->rows, 1);
-  const int64_t most = std::max<int64_t>(1, slots / (round * least));
-  const int64_t splits = std::max<int64_t>(1, std::min(want, most));
-  int64_t per = (slots + splits - 1) / splits;
-  per = (per + round - 1) / round * round;
-  return {(int)((slots + per - 1) / per), (int)per};
+  return (p->width + 2 * vec - 2) / vec;
 }
-Cut forward_cut(const mkg_logprob_params* p) { return cut_rows(p, 8, 1); }
-Cut backward_cut(const mkg_logprob_params* p) { return cut_rows(p, 8, 1); }
+Cut in_pieces(int64_t slots, int64_t piece, int threads) {
+  const int64_t splits = std::max<int64_t>((slots + piece / 2) / piece, 1);
+  int64_t per = (slots + splits - 1) / splits;
+  per = (per + threads - 1) / threads * threads;
+  return {(int)((slots + per - 1) / per), (int)per, threads};
+}
+// Pieces, not one share per resident block: SMs differ in speed, and 64 rows of 4,594,485 fp32 logits cut
+// into exactly as many blocks as are resident took 249 us forward and 432 us backward, against 211 us
+// (5.6 TB/s) and 345 us (6.8 TB/s, reading and writing) in pieces that are handed out as blocks end.
+// A piece costs the forward its ordering of alternatives (1,024 slots: 359 us, 8,192: 233 us) and the
+// backward its row's constants (256 slots: 642 us).
+constexpr int64_t kForwardPiece = 4096, kBackwardPiece = 2048;
+Cut forward_cut(const mkg_logprob_params* p) {
+  const int64_t slots = most_slots(p);
+  // enough rows to go round: 4,096 blocks need no joining (5 to 8 us with its launch)
+  if (p->rows >= 4096) return in_pieces(slots, slots, 128);
+  // about one row per SM: larger blocks instead of several and a join (256 x 17,050: 14 us, 30 us)
+  if (p->rows >= 128 && p->rows < 512 && slots < 8192) return in_pieces(slots, slots, 512);
+  const int64_t even = slots * p->rows / persistent_blocks(4);  // few rows: smaller pieces, to reach every SM
+  return in_pieces(slots, std::min(std::max<int64_t>(even, 1024), kForwardPiece), 128);
+}
+Cut backward_cut(const mkg_logprob_params* p) {
+  const int64_t slots = most_slots(p);
+  const int64_t even = slots * p->rows / persistent_blocks(8);
+  return in_pieces(slots, std::min(std::max<int64_t>(even, 512), kBackwardPiece), 128);
+}
 
 template <typename F> int by_type(int32_t dtype, bool mask, F f) {
   switch (dtype) {
@@ -601,15 +899,16 @@ template <typename F> int by_type(int32_t dtype, bool mask, F f) {
 template <typename T, bool kMask>
 int launch_narrow(const Rows& r, const void* logits, const uint8_t* mask, const int64_t* targets, const Outputs& o,
                   cudaStream_t st) {
-  const unsigned grid = (unsigned)((r.rows + kWarps - 1) / kWarps);
+  constexpr int kRows = kNarrowThreads / kWarp;
+  const unsigned grid = (unsigned)((r.rows + kRows - 1) / kRows);
   const T* x = static_cast<const T*>(logits);
-  const int per = (r.width + kWarp - 1) / kWarp;
-  if (per <= 1) logprob_narrow_kernel<T, kMask, 1><<<grid, kThreads, 0, st>>>(r, x, mask, targets, o);
-  else if (per <= 2) logprob_narrow_kernel<T, kMask, 2><<<grid, kThreads, 0, st>>>(r, x, mask, targets, o);
-  else if (per <= 4) logprob_narrow_kernel<T, kMask, 4><<<grid, kThreads, 0, st>>>(r, x, mask, targets, o);
-  else if (per <= 8) logprob_narrow_kernel<T, kMask, 8><<<grid, kThreads, 0, st>>>(r, x, mask, targets, o);
-  else if (per <= 16) logprob_narrow_kernel<T, kMask, 16><<<grid, kThreads, 0, st>>>(r, x, mask, targets, o);
-  else logprob_narrow_kernel<T, kMask, 32><<<grid, kThreads, 0, st>>>(r, x, mask, targets, o);
+  const int slots = ((r.width + 2 * kVec<T> - 2) / kVec<T> + kWarp - 1) / kWarp;  // of a lane, at most
+  if (slots <= 1) logprob_narrow_kernel<T, kMask, 1><<<grid, kNarrowThreads, 0, st>>>(r, x, mask, targets, o);
+  else if (slots <= 2) logprob_narrow_kernel<T, kMask, 2><<<grid, kNarrowThreads, 0, st>>>(r, x, mask, targets, o);
+  else if (slots <= 4) logprob_narrow_kernel<T, kMask, 4><<<grid, kNarrowThreads, 0, st>>>(r, x, mask, targets, o);
+  else if (kVec<T> == 8 || slots <= 8)
+    logprob_narrow_kernel<T, kMask, 8><<<grid, kNarrowThreads, 0, st>>>(r, x, mask, targets, o);
+  else logprob_narrow_kernel<T, kMask, 64 / kVec<T>><<<grid, kNarrowThreads, 0, st>>>(r, x, mask, targets, o);
   MKG_LAUNCHED("logprob_narrow_kernel");
   return MKG_OK;
 }
@@ -630,7 +929,7 @@ int logprob_forward(const mkg_logprob_params* p, const void* logits, const uint8
   Rows r;
   if (int rc = check_params(p, &r)) return rc;
   if (p->rows == 0) return MKG_OK;
-  MKG_REQUIRE(logits && entropy && lse && stats && (p->targets == 0 || (targets && logprobs)) &&
+  MKG_REQUIRE(logits && entropy && lse && (p->targets == 0 || (targets && logprobs)) &&
                   (p->topk == 0 || (top_ids && top_logprobs)), "logprob_forward: null argument");
   const size_t need = logprob_workspace_bytes(p);
   if (ws_bytes < need || (need > 0 && !ws)) {
@@ -649,17 +948,28 @@ int logprob_forward(const mkg_logprob_params* p, const void* logits, const uint8
     Partial* partials = static_cast<Partial*>(ws);
     unsigned long long* keys = reinterpret_cast<unsigned long long*>(partials + (cut.splits > 1 ? r.rows * cut.splits : 0));
     const unsigned grid = (unsigned)(r.rows * cut.splits);
-    if (r.topk > 0)
-      logprob_wide_kernel<T, kMask, true><<<grid, kThreads, 0, st>>>(r, x, mask, targets, o, cut.splits, cut.slots,
-                                                                     partials, keys);
-    else
-      logprob_wide_kernel<T, kMask, false><<<grid, kThreads, 0, st>>>(r, x, mask, targets, o, cut.splits, cut.slots,
-                                                                      partials, keys);
+    auto launch = [&](auto top, auto threads) {
+      constexpr int kT = decltype(threads)::value;
+      logprob_wide_kernel<T, kMask, decltype(top)::value, kT>
+          <<<grid, kT, 0, st>>>(r, x, mask, targets, o, cut.splits, cut.slots, partials, keys);
+    };
+    using Few = std::integral_constant<int, 128>;
+    using Many = std::integral_constant<int, 512>;
+    if (r.topk > 0) cut.threads == 128 ? launch(std::true_type(), Few()) : launch(std::true_type(), Many());
+    else cut.threads == 128 ? launch(std::false_type(), Few()) : launch(std::false_type(), Many());
     MKG_LAUNCHED("logprob_wide_kernel");
     if (cut.splits > 1) {
-      logprob_join_kernel<T, kMask><<<(unsigned)r.rows, kThreads, 0, st>>>(r, x, mask, targets, o, cut.splits,
-                                                                           partials, keys);
-      MKG_LAUNCHED("logprob_join_kernel");
+      cudaLaunchAttribute early;
+      early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+      early.val.programmaticStreamSerializationAllowed = 1;
+      cudaLaunchConfig_t config = {};
+      config.gridDim = dim3((unsigned)r.rows);
+      config.blockDim = dim3(kJoinThreads);
+      config.stream = st;
+      config.attrs = &early;
+      config.numAttrs = 1;
+      MKG_CUDA(cudaLaunchKernelEx(&config, logprob_join_kernel<T, kMask>, r, x, mask, targets, o, cut.splits,
+                                  (const Partial*)partials, (const unsigned long long*)keys));
     }
     return MKG_OK;
   });
@@ -680,10 +990,17 @@ int logprob_backward(const mkg_logprob_params* p, const void* logits, const uint
     const T* x = static_cast<const T*>(logits);
     MKG_REQUIRE(reinterpret_cast<uintptr_t>(x) % sizeof(T) == 0 && reinterpret_cast<uintptr_t>(grad) % sizeof(T) == 0,
                 "logprob_backward: misaligned tensors");
+    if (r.width <= kNarrow && r.targets + r.topk <= kNamedNarrow) {
+      constexpr int kRows = kNarrowThreads / kWarp;
+      logprob_backward_narrow_kernel<T, kMask><<<(unsigned)((r.rows + kRows - 1) / kRows), kNarrowThreads, 0, st>>>(
+          r, x, mask, u, static_cast<T*>(grad));
+      MKG_LAUNCHED("logprob_backward_narrow_kernel");
+      return MKG_OK;
+    }
     const Cut cut = backward_cut(p);
     MKG_REQUIRE(r.rows * cut.splits < (int64_t(1) << 31), "logprob_backward: too many rows");
     const size_t sh = (size_t)(r.targets + r.topk) * 8;
-    logprob_backward_kernel<T, kMask><<<(unsigned)(r.rows * cut.splits), kThreads, sh, st>>>(
+    logprob_backward_kernel<T, kMask, 128><<<(unsigned)(r.rows * cut.splits), 128, sh, st>>>(
         r, x, mask, u, static_cast<T*>(grad), cut.splits, cut.slots);
     MKG_LAUNCHED("logprob_backward_kernel");
     return MKG_OK;

@@ -30,48 +30,63 @@ class TargetLogprobs(NamedTuple):
     top_logprobs: torch.Tensor  # [..., topk] fp32, -inf padded
 
 
-def _rows(t: torch.Tensor, width: int, zero_ok: bool):
-    """(t as rows of unit column stride, their common stride in elements); copied only where the
-    leading dimensions have no common stride."""
-    if t.dim() == 1:
-        t = t.unsqueeze(0)
-    if zero_ok and t.numel() and all(st == 0 or n == 1 for st, n in zip(t.stride()[:-1], t.shape[:-1])) \
-            and (t.stride(-1) == 1 or width == 1):
-        return t, 0
-    if t.stride(-1) == 1 or width == 1:
-        try:
-            v = t.view(-1, width)
-            return v, v.stride(0) if v.shape[0] > 1 else width
-        except RuntimeError:
-            pass
-    t = t.contiguous()
-    return t.view(-1, width), width
+def _row_stride(t: torch.Tensor) -> int | None:
+    """Elements from one row of ``t`` [..., V] to the next; None where the rows have no common stride or
+    no unit column stride.  0 where there is one row, or one row stands for all."""
+    shape, strides = t.shape, t.stride()
+    if strides[-1] != 1 and shape[-1] != 1:
+        return None
+    step, rows = 0, 1
+    for n, st in zip(reversed(shape[:-1]), reversed(strides[:-1])):
+        if n == 1:
+            continue
+        if rows == 1:
+            step = st
+        elif st != step * rows:
+            return None
+        rows *= n
+    return step
+
+
+def _as_rows(t: torch.Tensor | None):
+    """(t, row stride) of a tensor the library can read, copied only where it cannot be read as it is."""
+    if t is None:
+        return None, 0
+    stride = _row_stride(t)
+    if stride is None:
+        t = t.contiguous()
+        stride = _row_stride(t)
+    return t, stride
+
+
+def _forward(logits, targets, mask, tau: float, topk: int, stats):
+    """(parameters, logprobs, entropy, lse, top_ids, top_logprobs); targets int64, contiguous; ``stats``
+    (fp32 [..., 2] or None) receives what the backward needs."""
+    lib, dev, lead = N.load(), logits.device, logits.shape[:-1]
+    x, stride = _as_rows(logits)
+    m, m_stride = _as_rows(mask)
+    rows = math.prod(lead)
+    p = N.LogprobParams(rows, logits.shape[-1], stride, m_stride, targets.shape[-1] if targets.dim() > len(lead) else 1,
+                        topk, tau, N.DTYPES[logits.dtype], 0)
+    logprobs = torch.empty(targets.shape, dtype=torch.float32, device=dev)
+    entropy, lse = (torch.empty(lead, dtype=torch.float32, device=dev) for _ in range(2))
+    top_ids = torch.empty((*lead, topk), dtype=torch.int64, device=dev)
+    top_logprobs = torch.empty((*lead, topk), dtype=torch.float32, device=dev)
+    with N.on_device(dev):
+        need = lib.mkg_logprob_workspace_bytes(p)
+        ws = N.workspace(need, dev) if need else None
+        N.check(lib.mkg_logprob_forward(p, x.data_ptr(), N.ptr(m), targets.data_ptr(), logprobs.data_ptr(),
+                                        entropy.data_ptr(), lse.data_ptr(), top_ids.data_ptr(),
+                                        top_logprobs.data_ptr(), N.ptr(stats), N.ptr(ws), need,
+                                        N.error_word(dev).data_ptr(), N.stream_handle(dev)), "logprob_forward")
+    return p, logprobs, entropy, lse, top_ids, top_logprobs
 
 
 class _TargetLogprobs(torch.autograd.Function):
-    """Flat form: logits [..., V], targets [N, S] int64, mask [..., V] uint8 or None."""
-
     @staticmethod
     def forward(ctx, logits, targets, mask, tau: float, topk: int):
-        lib = N.load()
-        dev, width = logits.device, int(logits.shape[-1])
-        x, stride = _rows(logits.detach(), width, False)
-        rows, s = int(targets.shape[0]), int(targets.shape[1])
-        m, m_stride = (None, 0) if mask is None else _rows(mask, width, True)
-        if stride < 0 or m_stride < 0:
-            raise ValueError("target_logprobs: negative strides")
-        p = N.LogprobParams(rows, width, stride, m_stride, s, topk, tau, N.DTYPES[x.dtype], 0)
-        f32 = dict(dtype=torch.float32, device=dev)
-        logprobs, top_logprobs = torch.empty((rows, s), **f32), torch.empty((rows, topk), **f32)
-        entropy, lse, stats = torch.empty(rows, **f32), torch.empty(rows, **f32), torch.empty((rows, 2), **f32)
-        top_ids = torch.empty((rows, topk), dtype=torch.int64, device=dev)
-        with torch.cuda.device(dev):
-            ws = N.workspace(lib.mkg_logprob_workspace_bytes(p), dev)
-            N.check(lib.mkg_logprob_forward(p, x.data_ptr(), N.ptr(m), targets.data_ptr(), logprobs.data_ptr(),
-                                            entropy.data_ptr(), lse.data_ptr(), top_ids.data_ptr(),
-                                            top_logprobs.data_ptr(), stats.data_ptr(), ws.data_ptr(), ws.numel(),
-                                            N.error_word(dev).data_ptr(), N.stream_handle(dev)), "logprob_forward")
-        ctx.p = p
+        stats = torch.empty((*logits.shape[:-1], 2), dtype=torch.float32, device=logits.device)
+        ctx.p, logprobs, entropy, lse, top_ids, top_logprobs = _forward(logits, targets, mask, tau, topk, stats)
         ctx.save_for_backward(logits, targets, mask, top_ids, entropy, stats)
         ctx.mark_non_differentiable(top_ids)
         ctx.set_materialize_grads(False)
@@ -81,15 +96,16 @@ class _TargetLogprobs(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, g_logprobs, g_entropy, g_lse, _g_ids, g_top):
         logits, targets, mask, top_ids, entropy, stats = ctx.saved_tensors
-        dev, p = logits.device, ctx.p
-        x, _ = _rows(logits.detach(), int(p.width), False)
-        m = None if mask is None else _rows(mask, int(p.width), True)[0]
-        ups = [None if g is None else g.to(torch.float32).contiguous() for g in (g_logprobs, g_entropy, g_lse, g_top)]
+        dev = logits.device
+        x, _ = _as_rows(logits)
+        m, _ = _as_rows(mask)
+        ups = [g if g is None or g.is_contiguous() else g.contiguous() for g in (g_logprobs, g_entropy, g_lse, g_top)]
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
-        with torch.cuda.device(dev):
-            N.check(N.load().mkg_logprob_backward(p, x.data_ptr(), N.ptr(m), targets.data_ptr(), top_ids.data_ptr(),
-                                                  entropy.data_ptr(), stats.data_ptr(), *(N.ptr(g) for g in ups),
-                                                  grad.data_ptr(), N.stream_handle(dev)), "logprob_backward")
+        with N.on_device(dev):
+            N.check(N.load().mkg_logprob_backward(ctx.p, x.data_ptr(), N.ptr(m), targets.data_ptr(),
+                                                  top_ids.data_ptr(), entropy.data_ptr(), stats.data_ptr(),
+                                                  *map(N.ptr, ups), grad.data_ptr(), N.stream_handle(dev)),
+                    "logprob_backward")
         return grad, None, None, None, None
 
 
@@ -123,8 +139,8 @@ def target_logprobs(logits: torch.Tensor, targets: torch.Tensor, tau: float = 1.
     if not 0 <= int(topk) <= N.LOGPROB_TOPK_MAX:
         raise ValueError(f"target_logprobs: topk must be in [0, {N.LOGPROB_TOPK_MAX}], got {topk}")
     tau = float(tau)
-    if not (tau > 0.0 and math.isfinite(tau)):
-        raise ValueError(f"target_logprobs: tau must be positive and finite, got {tau}")
+    if not 2.0 ** -60 <= tau <= 2.0 ** 60:
+        raise ValueError(f"target_logprobs: tau must be in [2^-60, 2^60], got {tau}")
     if mask is not None:
         if mask.dtype != torch.bool:
             raise TypeError(f"target_logprobs: mask must be bool, got {mask.dtype}")
@@ -136,9 +152,8 @@ def target_logprobs(logits: torch.Tensor, targets: torch.Tensor, tau: float = 1.
             N.require_cuda(t, what)
             if t.device != logits.device:
                 raise ValueError(f"target_logprobs: {what} on {t.device}, logits on {logits.device}")
-    rows = math.prod(lead)
-    t = targets.reshape(rows, s).to(torch.int64).contiguous()
+    t = targets.to(torch.int64).contiguous()
     m = None if mask is None else mask.view(torch.uint8)
-    lp, h, lse, ids, top = _TargetLogprobs.apply(logits, t, m, tau, int(topk))
-    k = (int(topk),)
-    return TargetLogprobs(lp.view(targets.shape), h.view(lead), lse.view(lead), ids.view(lead + k), top.view(lead + k))
+    if logits.requires_grad and torch.is_grad_enabled():
+        return TargetLogprobs(*_TargetLogprobs.apply(logits, t, m, tau, int(topk)))
+    return TargetLogprobs(*_forward(logits, t, m, tau, int(topk), None)[1:])

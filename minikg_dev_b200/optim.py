@@ -13,14 +13,29 @@ binades; a second moment above 0 is never held as 0.  Sums are taken in fp64 and
 """
 from __future__ import annotations
 
+import ctypes
 import math
+from itertools import accumulate
+from operator import attrgetter
 
-import numpy as np
 import torch
 
 from . import _native as N
 
+_dtype, _layout = attrgetter("dtype"), attrgetter("layout")
 _CODES = ("exp_avg_codes", "exp_avg_scale", "exp_avg_sq_codes", "exp_avg_sq_scale")
+
+
+class _Plan:
+    """Sizes, offsets into the flat moments and step-count indexes of a group's parameters."""
+
+    def __init__(self, numel, offset, index):
+        self.numel, self.offset, self.index = list(numel), list(offset), list(index)
+        table = ctypes.c_int64 * len(self.numel)
+        self.tables = tuple(table(*v) for v in (self.numel, self.offset, self.index))
+
+    def part(self, at) -> "_Plan":
+        return _Plan(*([v[i] for i in at] for v in (self.numel, self.offset, self.index)))
 
 
 class AdamW(torch.optim.Optimizer):
@@ -40,7 +55,7 @@ class AdamW(torch.optim.Optimizer):
         if state_bits not in (8, 32):
             raise ValueError(f"AdamW: state_bits must be 8 or 32, got {state_bits}")
         self.state_bits = int(state_bits)
-        self._plan = []     # per group: (numel, offset, index) int64 arrays over its parameters
+        self._plan = []     # a _Plan per group
         self._buffers = {}  # flat moments, scales, step counts, the ticket word
         self._total = self._tensors = 0
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
@@ -86,13 +101,12 @@ class AdamW(torch.optim.Optimizer):
 
     def _extend(self, params) -> None:
         """Room in the flat buffers for one more group; a graph captured before has to be captured again."""
-        numel = np.array([p.numel() for p in params], dtype=np.int64)
-        room = -(-numel // N.ADAMW_BLOCK) * N.ADAMW_BLOCK
-        offset = self._total + np.concatenate([[0], np.cumsum(room)[:-1]]).astype(np.int64)
-        index = self._tensors + np.arange(len(params), dtype=np.int64)
-        self._plan.append((numel, offset, index))
-        self._total += int(room.sum())
-        self._tensors += len(params)
+        numel = [p.numel() for p in params]
+        room = [-(-n // N.ADAMW_BLOCK) * N.ADAMW_BLOCK for n in numel]
+        offset = [self._total + x for x in accumulate(room, initial=0)][:-1]
+        self._plan.append(_Plan(numel, offset, range(self._tensors, self._tensors + len(numel))))
+        self._total += sum(room)
+        self._tensors += len(numel)
         if params:
             self._allocate(params[0].device)
 
@@ -113,8 +127,8 @@ class AdamW(torch.optim.Optimizer):
     def _views(self) -> None:
         """``state[p]``: each parameter's part of the flat buffers."""
         b = self._buffers
-        for group, (numel, offset, index) in zip(self.param_groups, self._plan):
-            for p, n, at, i in zip(group["params"], numel.tolist(), offset.tolist(), index.tolist()):
+        for group, plan in zip(self.param_groups, self._plan):
+            for p, n, at, i in zip(group["params"], plan.numel, plan.offset, plan.index):
                 if self.state_bits == 32:
                     moments = {k: b[k][at:at + n].view(p.shape) for k in ("exp_avg", "exp_avg_sq")}
                 else:
@@ -144,17 +158,19 @@ class AdamW(torch.optim.Optimizer):
             raise RuntimeError("AdamW: parameter groups are added with add_param_group")
         for group, plan in zip(self.param_groups, self._plan):
             params = group["params"]
-            if len(params) != len(plan[0]):
+            if len(params) != len(plan.numel):
                 raise RuntimeError("AdamW: a group's parameters changed after it was added")
             grads = [p.grad for p in params]
-            kinds = {(p.dtype, None if g is None else g.dtype) for p, g in zip(params, grads)}
-            if len(kinds) == 1 and None not in next(iter(kinds)):
-                self._launch(group, params, grads, *plan)
+            if any(g is None for g in grads):
+                at = [i for i, g in enumerate(grads) if g is not None]
+                params, grads, plan = [params[i] for i in at], [grads[i] for i in at], plan.part(at)
+            kinds = set(zip(map(_dtype, params), map(_dtype, grads)))
+            if len(kinds) == 1:
+                self._launch(group, params, grads, plan)
                 continue
             for kind in sorted(kinds, key=str):
-                at = [i for i, (p, g) in enumerate(zip(params, grads)) if g is not None and (p.dtype, g.dtype) == kind]
-                if at:
-                    self._launch(group, [params[i] for i in at], [grads[i] for i in at], *(a[at] for a in plan))
+                at = [i for i, (p, g) in enumerate(zip(params, grads)) if (p.dtype, g.dtype) == kind]
+                self._launch(group, [params[i] for i in at], [grads[i] for i in at], plan.part(at))
         return loss
 
     def load_kernels(self) -> None:
@@ -165,7 +181,7 @@ class AdamW(torch.optim.Optimizer):
                 if p.grad is None or (p.dtype, p.grad.dtype) in seen:
                     continue
                 seen.add((p.dtype, p.grad.dtype))
-                none = np.zeros(len(group["params"]), dtype=np.int64)
+                none = (ctypes.c_int64 * 1)()
                 self._call(group, p.dtype, p.grad.dtype, none, none, none, none, none)
 
     def _call(self, group, p_dtype, g_dtype, p_at, g_at, numel, offset, index) -> None:
@@ -176,31 +192,30 @@ class AdamW(torch.optim.Optimizer):
         hyper = N.AdamwParams(0.0 if on_device else float(lr), float(b1), float(b2), float(group["eps"]),
                               float(group["weight_decay"]), lr.data_ptr() if on_device else None, N.DTYPES[p_dtype],
                               N.DTYPES[g_dtype], self.state_bits, 0)
-        with torch.cuda.device(dev):
-            N.check(N.load().mkg_adamw_step(hyper, self._state_struct(), len(numel), p_at.ctypes.data, g_at.ctypes.data,
-                                            numel.ctypes.data, offset.ctypes.data, index.ctypes.data,
+        with N.on_device(dev):
+            N.check(N.load().mkg_adamw_step(hyper, self._state_struct(), len(numel), p_at, g_at, numel, offset, index,
                                             N.stream_handle(dev)), "adamw_step")
 
-    def _launch(self, group, params, grads, numel, offset, index) -> None:
+    def _launch(self, group, params, grads, plan) -> None:
         dev = self._buffers["steps"].device
         n, dtypes = len(params), (params[0].dtype, grads[0].dtype)
         if dtypes[0] not in N.DTYPES or dtypes[1] not in N.DTYPES:
             raise TypeError(f"AdamW: parameters of {dtypes[0]} with gradients of {dtypes[1]}")
-        if not all(g.layout == torch.strided for g in grads):
+        if set(map(_layout, grads)) != {torch.strided}:
             raise RuntimeError("AdamW: gradients must be dense")
         if not all(map(torch.Tensor.is_contiguous, grads)):
             grads = [g.contiguous() for g in grads]
-        own = numel.tolist()
-        if (list(map(torch.Tensor.numel, params)) != own or list(map(torch.Tensor.numel, grads)) != own
+        if (list(map(torch.Tensor.numel, params)) != plan.numel or list(map(torch.Tensor.numel, grads)) != plan.numel
                 or not all(map(torch.Tensor.is_contiguous, params))):
             raise RuntimeError("AdamW: a parameter changed its size or layout, or its gradient has another size")
         where = set(map(torch.Tensor.get_device, params))
         where.update(map(torch.Tensor.get_device, grads))
         if where != {dev.index}:
             raise RuntimeError(f"AdamW: parameters and gradients must be on {dev}")
-        p_at = np.fromiter(map(torch.Tensor.data_ptr, params), np.int64, n)
-        g_at = np.fromiter(map(torch.Tensor.data_ptr, grads), np.int64, n)
-        self._call(group, *dtypes, p_at, g_at, numel, offset, index)
+        table = ctypes.c_int64 * n
+        p_at = table(*map(torch.Tensor.data_ptr, params))
+        g_at = table(*map(torch.Tensor.data_ptr, grads))
+        self._call(group, *dtypes, p_at, g_at, *plan.tables)
         torch.autograd.graph.increment_version(params)
 
     # ------------------------------------------------------------------ the moments
@@ -217,7 +232,7 @@ class AdamW(torch.optim.Optimizer):
     def _unpacked(self, buffers):
         dev = buffers["steps"].device
         m, v = (torch.empty(max(self._total, 1), dtype=torch.float32, device=dev) for _ in range(2))
-        with torch.cuda.device(dev):
+        with N.on_device(dev):
             N.check(N.load().mkg_adamw_unpack(self._state_struct(buffers), m.data_ptr(), v.data_ptr(),
                                               N.stream_handle(dev)), "adamw_unpack")
         return m[:self._total], v[:self._total]
@@ -239,7 +254,7 @@ class AdamW(torch.optim.Optimizer):
             return
         entries = []
         for group, new, plan in zip(self.param_groups, groups, self._plan):
-            for p, key, n, at, i in zip(group["params"], new["params"], *(a.tolist() for a in plan)):
+            for p, key, n, at, i in zip(group["params"], new["params"], plan.numel, plan.offset, plan.index):
                 e = state_dict["state"].get(key)
                 if e is None:
                     continue
@@ -276,7 +291,7 @@ class AdamW(torch.optim.Optimizer):
             self._buffers["exp_avg"][:self._total].copy_(m[:self._total])
             self._buffers["exp_avg_sq"][:self._total].copy_(v[:self._total])
         else:
-            with torch.cuda.device(dev):
+            with N.on_device(dev):
                 N.check(N.load().mkg_adamw_pack(self._state_struct(), m.data_ptr(), v.data_ptr(),
                                                 N.stream_handle(dev)), "adamw_pack")
         for have, new in zip(self.param_groups, groups):
