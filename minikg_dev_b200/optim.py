@@ -260,6 +260,8 @@ class AdamW(torch.optim.Optimizer):
                     continue
                 if "exp_avg" not in e and _CODES[0] not in e:
                     raise ValueError("AdamW: a state dict entry without moments")
+                if "exp_avg" in e and bool((e["exp_avg_sq"] < 0).any()):
+                    raise ValueError("AdamW: a state dict entry with negative second moments")
                 if e["exp_avg" if "exp_avg" in e else _CODES[0]].numel() != n:
                     raise ValueError("AdamW: a state dict entry of another size")
                 entries.append((e, n, at, i))
