@@ -15,6 +15,7 @@ from __future__ import annotations
 import numpy as np
 import torch
 
+from .logprobs import TargetLogprobs, target_logprobs
 from .proof import decode_topk, kernel_sparse_scores, sparse_topk
 
 _TOPK_KERNEL_MAX = 1024  # kTopkMax of mkg_decode_topk
@@ -45,6 +46,28 @@ def ordered_candidates(raw: torch.Tensor, cap: int = 0):
         return (torch.full((B, 0), -1, dtype=torch.int64, device=dev), torch.zeros((B, 0), device=dev),
                 torch.zeros(B, dtype=torch.int64, device=dev))
     return sparse_topk(keys, vals.float(), B, E, k)
+
+
+def tail_logprobs(raw: torch.Tensor, tails: torch.Tensor, mask: torch.Tensor | None = None,
+                  topk: int = 0) -> TargetLogprobs:
+    """Log probabilities of given tails among each query's answers: raw scores ``[B, E]`` (dense, or sparse
+    COO) as weights, ``p = raw / sum of raw`` over the entities with a positive score and, if given, a True
+    ``mask`` ([B, E] or [E]: False filters an entity out, as known answers are when another is ranked).
+
+    ``tails [B]`` or ``[B, S]`` (-1 padded); alternatives are ordered by the fp32 logarithm of their scores
+    (which may bring two neighbouring scores to a tie); the other outputs are those of ``logprobs.target_logprobs``: a
+    tail without a positive score has log probability -inf.  ``-tail_logprobs(...).logprobs`` of the true
+    tails is a loss on the scores: gradients flow to ``raw``."""
+    if raw.dim() != 2:
+        raise ValueError(f"tail_logprobs: raw must be [B, E], got {tuple(raw.shape)}")
+    raw = (raw.to_dense() if raw.is_sparse else raw).float()
+    scored = ~(raw <= 0)  # a NaN score stays a candidate, and is seen
+    if mask is not None:
+        if mask.dtype != torch.bool:
+            raise TypeError(f"tail_logprobs: mask must be bool, got {mask.dtype}")
+        scored = scored & mask
+    # below the least normal score log would be -inf and its gradient 0 * inf: those are no candidates
+    return target_logprobs(raw.clamp_min(torch.finfo(torch.float32).tiny).log(), tails, 1.0, scored, topk)
 
 
 def candidate_rows(tails: torch.Tensor, scores: torch.Tensor, counts: torch.Tensor) -> dict:

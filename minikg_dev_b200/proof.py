@@ -28,6 +28,7 @@ import torch
 from . import _native as N
 from .fastlog_kernel import HopRange
 from .graph import DeviceGraph, build_csr_structure
+from .optim import AdamW
 from .rules import rule_weights
 from .sparse_reducers import (max_sp_3d, normalize_sparse3d, prune_sparse3d_active_entities, sparse3d_max, sum_sp_3d,
                               sum_sparse3d_concat)
@@ -125,8 +126,9 @@ class ProofRunner:
         return grad_w, (grad_edge if want_edge_grad else None)
 
     def capture(self, heads, w_hops, out, msgs, grad_out, edge_scores, grad_w, grad_edge=None, mask=None,
-                is_score: bool = True, scale: float = 1.0, host_inputs=(), host_outputs=()) -> "torch.cuda.CUDAGraph":
-        """One training step (edge-factor refresh, forward, backward) captured as a CUDA graph
+                is_score: bool = True, scale: float = 1.0, host_inputs=(), host_outputs=(),
+                optimizer=None) -> "torch.cuda.CUDAGraph":
+        """One training step (edge-factor refresh, forward, backward, update) captured as a CUDA graph
         over these buffers.  Write new inputs into ``heads`` / ``w_hops`` / ``edge_scores`` /
         ``grad_out`` (and ``mask``) in place, then ``graph.replay()`` reruns the step with no
         host work; results land in ``out``, ``msgs``, ``grad_w``, ``grad_edge``.  The library
@@ -135,7 +137,11 @@ class ProofRunner:
         ``host_inputs``: (device tensor, pinned host tensor) pairs copied host to device at the
         start of every replay, so new inputs can be written into the host tensors instead;
         ``host_outputs``: (pinned host tensor, device tensor) pairs copied device to host at its
-        end (read them after a synchronisation of the replaying stream)."""
+        end (read them after a synchronisation of the replaying stream).
+
+        ``optimizer``: an ``optim.AdamW`` over ``edge_scores`` and / or ``w_hops`` (``torch.nn.Parameter``s
+        whose ``.grad`` is ``grad_edge`` / ``grad_w``), stepped after the backward of every replay.
+        Capturing takes no step.  A tensor ``lr`` is read at each replay, a number is kept as it is."""
         dev = self.graph.device
         for name, t, dt in (("heads", heads, torch.int64), ("w_hops", w_hops, torch.float32),
                             ("out", out, torch.float32), ("msgs", msgs, torch.int64),
@@ -152,25 +158,41 @@ class ProofRunner:
                     raise ValueError(f"capture: {kind} pairs a contiguous tensor on {dev} with a pinned "
                                      "host tensor of the same shape and dtype")
         want_edge = grad_edge is not None
+        if optimizer is not None:
+            if not isinstance(optimizer, AdamW):
+                raise ValueError("capture: optimizer must be an optim.AdamW")
+            pairs = {(t.data_ptr(), g.data_ptr(), t.numel()) for t, g in ((w_hops, grad_w), (edge_scores, grad_edge))
+                     if g is not None}
+            for p in (p for group in optimizer.param_groups for p in group["params"]):
+                if p.grad is None or (p.data_ptr(), p.grad.data_ptr(), p.numel()) not in pairs \
+                        or p.grad.numel() != p.numel():
+                    raise ValueError("capture: the optimizer's parameters must be w_hops with gradient grad_w or "
+                                     "edge_scores with gradient grad_edge")
 
-        def step():
+        def step(update: bool):
             for d, h in host_inputs:
                 d.copy_(h, non_blocking=True)
             self.graph.set_edge_factor(mask, edge_scores, is_score, scale)
             self.forward(heads, w_hops, out, msgs)
             self.backward(grad_out, mask, edge_scores, is_score, scale, want_edge, grad_w, grad_edge)
+            if update:
+                optimizer.step()
             for h, d in host_outputs:
                 h.copy_(d, non_blocking=True)
 
         side = torch.cuda.Stream(dev)
         side.wait_stream(torch.cuda.current_stream(dev))
         with torch.cuda.stream(side):
-            step()  # warm-up outside the capture (lazy adjacency, kernel attributes)
+            step(False)  # warm-up outside the capture (lazy adjacency, kernel attributes)
+            if optimizer is not None:
+                optimizer.load_kernels()
         torch.cuda.current_stream(dev).wait_stream(side)
         torch.cuda.synchronize(dev)
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
-            step()
+            step(optimizer is not None)
+        # what the replays use besides the caller's buffers lives as long as the graph
+        graph.keep = (self, optimizer, mask, edge_scores, list(self._keep))
         return graph
 
     def row_activity(self, hop: int) -> torch.Tensor:

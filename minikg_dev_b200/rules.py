@@ -16,14 +16,20 @@ Everything depends on the query only through its target relation, so here:
   (``mkg_rule_softmax_forward``: [K, B, L, n], the layout the hop loop consumes), backward
   summed over each relation's queries in a fixed order (``mkg_rule_softmax_backward``).
 
+``rule_logprobs`` reads the rules rather than running them: log probabilities of given rule bodies,
+the entropy of each rule's channel distributions and its best channels (``logprobs.target_logprobs``).
+
 Kernels flag an out-of-range relation in the device error word (raised by the next checked
 call, ``_native.raise_device_errors``); the product path has no CPU implementation.
 """
 from __future__ import annotations
 
+from typing import NamedTuple
+
 import torch
 
 from . import _native as N
+from .logprobs import target_logprobs
 
 
 def _params(n: int, H: int, L: int, K: int, U: int, B: int = 1, tau: float = 1.0) -> N.RuleParams:
@@ -222,3 +228,55 @@ def rule_weights_from_logits(logits: torch.Tensor, tau: float) -> torch.Tensor:
     ar = torch.arange(B, dtype=torch.int64, device=logits.device)
     qptr = torch.arange(B + 1, dtype=torch.int64, device=logits.device)
     return RuleSoftmax.apply(logits, ar, qptr, ar, float(tau))
+
+
+# ------------------------------------------------------------------ reading rules
+class RuleLogprobs(NamedTuple):
+    logprobs: torch.Tensor      # [B, S, L] fp32: log probability of body s under rule l
+    entropy: torch.Tensor       # [B, K, L] fp32: of each hop's channel distribution
+    top_channels: torch.Tensor  # [B, K, L, topk] int64, -1 padded
+    top_logprobs: torch.Tensor  # [B, K, L, topk] fp32
+
+
+def rule_logprobs(model, target_rel: torch.Tensor, bodies: torch.Tensor, tau: float | None = None,
+                  topk: int = 0) -> RuleLogprobs:
+    """Log probabilities of rule bodies under the rules of each query's target relation.
+
+    ``target_rel [B]``; ``bodies [B, S, K]`` int64 / int32: the channel that body s of query b takes at
+    each hop (-1: the hop is left out, so a body of -1 is padding and has log probability 0).  A body's
+    log probability under rule l is the sum over the hops of log softmax(logits[hop, l] / tau) at its
+    channel, the product that the hop loop gives each of its paths.  Runs once per distinct relation, on
+    the logits of ``build_rule_logits``; gradients flow to every producer parameter through the log
+    probabilities and the entropy, in a fixed order."""
+    tau = float(model.tau_1 if tau is None else tau)
+    if bodies.dim() != 3 or bodies.shape[0] != target_rel.numel():
+        raise ValueError(f"rule_logprobs: bodies must be [{target_rel.numel()}, S, K], got {tuple(bodies.shape)}")
+    if bodies.dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"rule_logprobs: bodies must be int64 or int32, got {bodies.dtype}")
+    if has_lstm_producer(model):
+        rel_u, query_u, qptr, qperm = group_queries(target_rel)
+        logits = relation_rule_logits(model, rel_u)
+    else:  # a model with its own producer: one row of logits per query
+        logits = model.build_rule_logits(target_rel)
+        query_u = qperm = torch.arange(target_rel.numel(), device=logits.device)
+        qptr = torch.arange(target_rel.numel() + 1, device=logits.device)
+    U, K, L, _ = (int(x) for x in logits.shape)
+    B, S = int(bodies.shape[0]), int(bodies.shape[1])
+    if int(bodies.shape[2]) != K:
+        raise ValueError(f"rule_logprobs: bodies have {int(bodies.shape[2])} hops, the rules {K}")
+    # the bodies of a relation's queries side by side: rank = a query's place among them
+    rank = torch.empty_like(query_u)
+    rank[qperm] = torch.arange(B, device=query_u.device) - qptr[query_u[qperm]]
+    Q = int((qptr[1:] - qptr[:-1]).max()) if B else 0
+    placed = torch.full((U, Q, S, K), -1, dtype=torch.int64, device=logits.device)
+    placed[query_u, rank] = bodies.to(device=logits.device, dtype=torch.int64)
+    placed = placed.view(U, Q * S, K).permute(0, 2, 1)[:, :, None, :].expand(U, K, L, Q * S)
+    parts, entropy, ids, top = [], None, None, None
+    for at in range(0, max(Q * S, 1), N.LOGPROB_TARGETS_MAX):
+        out = target_logprobs(logits, placed[..., at:at + N.LOGPROB_TARGETS_MAX], tau, topk=topk if at == 0 else 0)
+        parts.append(out.logprobs.sum(1))
+        if at == 0:
+            entropy, ids, top = out.entropy, out.top_ids, out.top_logprobs
+    per_rule = (parts[0] if len(parts) == 1 else torch.cat(parts, -1)).view(U, L, Q, S)
+    lp = per_rule[query_u, :, rank].transpose(1, 2)
+    return RuleLogprobs(lp, entropy[query_u], ids[query_u], top[query_u])
