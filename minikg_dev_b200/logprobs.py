@@ -48,6 +48,10 @@ def _row_stride(t: torch.Tensor) -> int | None:
     return step
 
 
+def _strides(size) -> tuple[int, ...]:
+    return tuple(math.prod(size[i + 1:]) for i in range(len(size)))
+
+
 def _as_rows(t: torch.Tensor | None):
     """(t, row stride) of a tensor the library can read, copied only where it cannot be read as it is."""
     if t is None:
@@ -68,10 +72,17 @@ def _forward(logits, targets, mask, tau: float, topk: int, stats):
     rows = math.prod(lead)
     p = N.LogprobParams(rows, logits.shape[-1], stride, m_stride, targets.shape[-1] if targets.dim() > len(lead) else 1,
                         topk, tau, N.DTYPES[logits.dtype], 0)
-    logprobs = torch.empty(targets.shape, dtype=torch.float32, device=dev)
-    entropy, lse = (torch.empty(lead, dtype=torch.float32, device=dev) for _ in range(2))
+    if stats is None:  # nobody differentiates: one allocation, the outputs are its parts
+        s, k = targets.numel(), rows * topk
+        buffer = torch.empty(s + 2 * rows + k, dtype=torch.float32, device=dev)
+        logprobs, entropy, lse, top_logprobs = (
+            torch.as_strided(buffer, size, _strides(size), at)
+            for size, at in ((targets.shape, 0), (lead, s), (lead, s + rows), ((*lead, topk), s + 2 * rows)))
+    else:
+        logprobs = torch.empty_like(targets, dtype=torch.float32)
+        entropy, lse = (torch.empty(lead, dtype=torch.float32, device=dev) for _ in range(2))
+        top_logprobs = torch.empty((*lead, topk), dtype=torch.float32, device=dev)
     top_ids = torch.empty((*lead, topk), dtype=torch.int64, device=dev)
-    top_logprobs = torch.empty((*lead, topk), dtype=torch.float32, device=dev)
     with N.on_device(dev):
         need = lib.mkg_logprob_workspace_bytes(p)
         ws = N.workspace(need, dev) if need else None

@@ -148,7 +148,6 @@ class AdamW(torch.optim.Optimizer):
         return self.__dict__.copy()
 
     # ------------------------------------------------------------------ the step
-    @torch.no_grad()
     def step(self, closure=None):
         loss = None
         if closure is not None:
@@ -204,7 +203,7 @@ class AdamW(torch.optim.Optimizer):
         if set(map(_layout, grads)) != {torch.strided}:
             raise RuntimeError("AdamW: gradients must be dense")
         if not all(map(torch.Tensor.is_contiguous, grads)):
-            grads = [g.contiguous() for g in grads]
+            grads = [g.detach().contiguous() for g in grads]
         if (list(map(torch.Tensor.numel, params)) != plan.numel or list(map(torch.Tensor.numel, grads)) != plan.numel
                 or not all(map(torch.Tensor.is_contiguous, params))):
             raise RuntimeError("AdamW: a parameter changed its size or layout, or its gradient has another size")
