@@ -35,7 +35,7 @@ constexpr int kBlock = MKG_ADAMW_BLOCK;      // values that share a scale: a war
 constexpr int kQuad = 4;                     // values per access
 constexpr int kQuads = kBlock / kQuad / kWarp;  // accesses per thread
 constexpr int kChunk = kThreads / kWarp * kBlock;
-constexpr int kBlocks8 = 4, kBlocks32 = 5;   // blocks per SM
+constexpr int kBlocks8 = 3, kBlocks32 = 5;   // blocks per SM
 constexpr unsigned kFull = 0xffffffffu;
 constexpr int kFirstLow = -120, kFirstHigh = 119, kSecondLow = -90, kSecondHigh = 120;  // of the blocks' scales
 
@@ -85,13 +85,14 @@ template <> struct Bits<float> { using type = uint4; };
 template <> struct Bits<__nv_bfloat16> { using type = uint2; };
 template <> struct Bits<__half> { using type = uint2; };
 
-template <typename T> __device__ __forceinline__ void load_quad(const T* at, float (&out)[kQuad]) {
-  using B = typename Bits<T>::type;
-  const B raw = *reinterpret_cast<const B*>(at);
+template <typename T> __device__ __forceinline__ void spread(const typename Bits<T>::type& raw, float (&out)[kQuad]) {
   T e[kQuad];
   memcpy(e, &raw, sizeof(raw));
 #pragma unroll
   for (int i = 0; i < kQuad; ++i) out[i] = to_f32<T>(e[i]);
+}
+template <typename T> __device__ __forceinline__ void load_quad(const T* at, float (&out)[kQuad]) {
+  spread<T>(*reinterpret_cast<const typename Bits<T>::type*>(at), out);
 }
 template <typename T> __device__ __forceinline__ void store_quad(T* at, const float (&v)[kQuad]) {
   T e[kQuad];
@@ -102,6 +103,14 @@ template <typename T> __device__ __forceinline__ void store_quad(T* at, const fl
   memcpy(&raw, e, sizeof(raw));
   *reinterpret_cast<B*>(at) = raw;
 }
+// A lane's share of a whole block as it is in memory, moments in 8 bits: what a warp loads for its next
+// block while it works on this one.
+template <typename P, typename G> struct Share {
+  typename Bits<P>::type p[kQuads];
+  typename Bits<G>::type g[kQuads];
+  uint32_t first[kQuads], second[kQuads];
+  float first_scale, second_scale;
+};
 // A lane's share of a block of a tensor: `left` values from `at` on exist, others read as 0.  whole: all
 // 256 do, and `at` is aligned for loads of four.
 template <typename T>
@@ -367,6 +376,8 @@ __global__ void __launch_bounds__(kThreads, k8 ? kBlocks8 : kBlocks32) adamw_ker
   const int chunks = t.chunk[t.n];
   int known = -1, turn = 0;
   const bool plain = h.eps >= 0x1p-60f;
+  Share<P, G> next;    // moments in 8 bits
+  bool ready = false;  // next holds the block that comes
   const int end = min((static_cast<int>(blockIdx.x) + 1) * run, chunks);
   for (int chunk = blockIdx.x * run; chunk < end; ++chunk) {
     const int e = tensor_of(t, chunk);
@@ -398,25 +409,59 @@ __global__ void __launch_bounds__(kThreads, k8 ? kBlocks8 : kBlocks32) adamw_ker
                        reinterpret_cast<uintptr_t>(g) % (kQuad * sizeof(G)) == 0;
     float pv[kQuads][kQuad], gv[kQuads][kQuad], mv[kQuads][kQuad], vv[kQuads][kQuad];
     float fs = 0.0f, ss = 0.0f;
-    if (any) {
-      if constexpr (k8) {
-        const uint32_t* first = static_cast<uint32_t*>(s.first) + block * (kBlock / kQuad);
-        const uint32_t* second = static_cast<uint32_t*>(s.second) + block * (kBlock / kQuad);
-        fs = s.first_scale[block];
-        ss = s.second_scale[block];
+    if constexpr (k8) {
+      if (any) {
+        const uint32_t* first = static_cast<uint32_t*>(s.first) + block * (kBlock / kQuad) + lane;
+        const uint32_t* second = static_cast<uint32_t*>(s.second) + block * (kBlock / kQuad) + lane;
+        auto fetch = [&](int64_t ahead) {  // `ahead` blocks further on
 #pragma unroll
-        for (int u = 0; u < kQuads; ++u) {
-          decode_first(first[u * kWarp + lane], fs, mv[u]);
-          decode_second(second[u * kWarp + lane], ss, vv[u]);
+          for (int u = 0; u < kQuads; ++u) {
+            const int64_t j = ahead * kBlock + (u * kWarp + lane) * kQuad;
+            next.p[u] = *reinterpret_cast<const typename Bits<P>::type*>(p + j);
+            next.g[u] = *reinterpret_cast<const typename Bits<G>::type*>(g + j);
+            next.first[u] = first[ahead * (kBlock / kQuad) + u * kWarp];
+            next.second[u] = second[ahead * (kBlock / kQuad) + u * kWarp];
+          }
+          next.first_scale = s.first_scale[block + ahead];
+          next.second_scale = s.second_scale[block + ahead];
+        };
+        if (whole) {
+          if (!ready) fetch(0);
+          fs = next.first_scale;
+          ss = next.second_scale;
+#pragma unroll
+          for (int u = 0; u < kQuads; ++u) {
+            spread<P>(next.p[u], pv[u]);
+            spread<G>(next.g[u], gv[u]);
+            decode_first(next.first[u], fs, mv[u]);
+            decode_second(next.second[u], ss, vv[u]);
+          }
+          // the same warp's block of the next chunk, if that is whole and the same tensor's
+          ready = chunk + 1 < end && left - kChunk >= kBlock;
+          if (ready) fetch(kChunk / kBlock);
+        } else {
+          ready = false;
+          fs = s.first_scale[block];
+          ss = s.second_scale[block];
+#pragma unroll
+          for (int u = 0; u < kQuads; ++u) {
+            decode_first(first[u * kWarp], fs, mv[u]);
+            decode_second(second[u * kWarp], ss, vv[u]);
+          }
+          load_block(p, left, false, lane, pv);
+          load_block(g, left, false, lane, gv);
         }
-      } else {
+      }
+    }
+    if (any) {
+      if constexpr (!k8) {
         const float* first = static_cast<float*>(s.first) + block * kBlock;
         const float* second = static_cast<float*>(s.second) + block * kBlock;
         load_block(first, kBlock, true, lane, mv);
         load_block(second, kBlock, true, lane, vv);
+        load_block(p, left, whole, lane, pv);
+        load_block(g, left, whole, lane, gv);
       }
-      load_block(p, left, whole, lane, pv);
-      load_block(g, left, whole, lane, gv);
       if constexpr (k8) {
         const Held at{static_cast<uint32_t*>(s.first) + block * (kBlock / kQuad) + lane,
                       static_cast<uint32_t*>(s.second) + block * (kBlock / kQuad) + lane, s.first_scale + block,

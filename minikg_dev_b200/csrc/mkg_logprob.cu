@@ -196,19 +196,22 @@ __device__ __forceinline__ unsigned long long exchange(unsigned long long v, int
   const unsigned long long w = shfl_xor64(v, o);
   return (w > v) == up ? w : v;
 }
-// The 32 keys of a warp in ascending order of the lanes.
+// The keys of every kLanes lanes of a warp in ascending order of the lanes.
+template <int kLanes = kWarp>
 __device__ __forceinline__ unsigned long long sort_ascending(unsigned long long v, int lane) {
 #pragma unroll
-  for (int size = 2; size <= 32; size <<= 1)
+  for (int size = 2; size <= kLanes; size <<= 1)
 #pragma unroll
-    for (int o = size >> 1; o > 0; o >>= 1) v = exchange(v, o, ((lane & o) != 0) == ((lane & size) == 0 || size == 32));
+    for (int o = size >> 1; o > 0; o >>= 1)
+      v = exchange(v, o, ((lane & o) != 0) == ((lane & size) == 0 || size == kLanes));
   return v;
 }
-// `best` descending over the lanes, `add` ascending: the 32 largest of both, descending.
+// `best` descending over kLanes lanes, `add` ascending: the kLanes largest of both, descending.
+template <int kLanes = kWarp>
 __device__ __forceinline__ unsigned long long merge_best(unsigned long long best, unsigned long long add, int lane) {
   unsigned long long v = best > add ? best : add;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = exchange(v, o, (lane & o) == 0);
+  for (int o = kLanes / 2; o > 0; o >>= 1) v = exchange(v, o, (lane & o) == 0);
   return v;
 }
 
@@ -315,23 +318,41 @@ __device__ __forceinline__ unsigned long long merge_list(unsigned long long best
   return best;
 }
 
-// ---------------------------------------------------------------- narrow rows: a warp each
-template <typename T, bool kMask, int kSlots>
+// ---------------------------------------------------------------- narrow rows: a warp, or eight lanes each
+// Rows of about a hundred columns keep only a quarter of a warp busy with columns, and what a row costs
+// besides (sums over the lanes, ordering, outputs: about 800 instructions of a warp) is shared by four of
+// them: 65,536 rows of 103 fp32 logits with 5 alternatives took 60 us forward and 53 us backward with a
+// warp each, 29 and 25 us with eight lanes.
+template <int kLanes> __device__ __forceinline__ float lanes_max(float v) {
+#pragma unroll
+  for (int o = kLanes / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kFull, v, o));
+  return v;
+}
+template <int kLanes> __device__ __forceinline__ float lanes_sum(float v) {
+#pragma unroll
+  for (int o = kLanes / 2; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
+  return v;
+}
+
+template <typename T, bool kMask, int kSlots, int kLanes>
 __global__ void __launch_bounds__(kNarrowThreads) logprob_narrow_kernel(Rows r, const T* __restrict__ logits,
                                                                         const uint8_t* __restrict__ masks,
                                                                         const int64_t* __restrict__ targets, Outputs o) {
-  __shared__ unsigned long long sh_cand[kNarrowThreads / kWarp][2 * kWarp];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kNarrowThreads / kWarp) + warp;
-  if (row >= r.rows) return;
+  constexpr int kRows = kNarrowThreads / kLanes, kRoom = 2 * kLanes;
+  __shared__ unsigned long long sh_cand[kRows][kRoom];
+  const int lane = threadIdx.x & 31, part = lane % kLanes, own = threadIdx.x / kLanes;
+  int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + own;
+  if (row - lane / kLanes >= r.rows) return;  // the whole warp is past the end
+  const bool valid = row < r.rows;  // others of the warp repeat the last row and write nothing
+  row = min(row, r.rows - 1);
   const T* x = logits + row * r.stride;
   const uint8_t* mask = kMask ? masks + row * r.mask_stride : nullptr;
   const RowView<T> view(x, mask, r.width);
-  const Target target = read_target<T>(r, targets, row, lane, x, mask);
+  const Target target = read_target<T>(r, targets, row, part, x, mask);
   float v[kSlots][kVec<T>];
 #pragma unroll
   for (int q = 0; q < kSlots; ++q) {
-    const int slot = q * kWarp + lane;
+    const int slot = q * kLanes + part;
     if (slot < view.slots) {
       view.template load<kMask>(slot, v[q]);
     } else {
@@ -347,11 +368,10 @@ __global__ void __launch_bounds__(kNarrowThreads) logprob_narrow_kernel(Rows r, 
     for (int i = 0; i < kVec<T>; ++i)
       if (v[q][i] > a.m) {
         a.m = v[q][i];
-        at = view.first(q * kWarp + lane) + i;
+        at = view.first(q * kLanes + part) + i;
       }
   const unsigned long long mine = a.m > -kInf ? rank_key(a.m, static_cast<uint32_t>(at)) : 0;
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) a.m = fmaxf(a.m, __shfl_xor_sync(kFull, a.m, off));
+  a.m = lanes_max<kLanes>(a.m);
   const float from = a.m == -kInf ? 0.0f : a.m;
 #pragma unroll
   for (int q = 0; q < kSlots; ++q)
@@ -362,41 +382,45 @@ __global__ void __launch_bounds__(kNarrowThreads) logprob_narrow_kernel(Rows r, 
       a.s += e;
       a.t = fmaf(e, y, a.t);
     }
-  a.s = warp_sum(a.s);
-  a.t = warp_sum(a.t);
+  a.s = lanes_sum<kLanes>(a.s);
+  a.t = lanes_sum<kLanes>(a.t);
   unsigned long long best = 0;
   if (r.topk > 0) {
     // elements below the topk-th largest of the lanes' maxima have topk better ones
-    const unsigned long long sorted = sort_ascending(mine, lane);
-    const unsigned long long floor = __shfl_sync(kFull, sorted, 32 - r.topk);
+    const unsigned long long sorted = sort_ascending<kLanes>(mine, lane);
+    const unsigned long long floor = __shfl_sync(kFull, sorted, lane - part + kLanes - r.topk);
     const float least = floor ? packed_value(floor) : -kInf;
     const int least_at = floor ? static_cast<int>(packed_rank(floor)) : 0x7fffffff;
-    unsigned long long* cand = sh_cand[warp];
+    unsigned long long* cand = sh_cand[own];
+    const unsigned before = ((1u << part) - 1) << (lane - part);  // the row's lanes before this one
+    const unsigned row_lanes = (kLanes == kWarp ? kFull : (1u << (kLanes & 31)) - 1) << (lane - part);
     int n = 0;
 #pragma unroll
     for (int q = 0; q < kSlots; ++q)
 #pragma unroll
       for (int i = 0; i < kVec<T>; ++i) {
-        const int j = view.first(q * kWarp + lane) + i;
+        const int j = view.first(q * kLanes + part) + i;
         const bool in = v[q][i] > least || (v[q][i] == least && v[q][i] > -kInf && j <= least_at);
         const unsigned who = __ballot_sync(kFull, in);
-        const int to = n + __popc(who & ((1u << lane) - 1));
-        if (in && to < 2 * kWarp) cand[to] = rank_key(v[q][i], static_cast<uint32_t>(j));
-        n += __popc(who);
+        const int to = n + __popc(who & before);
+        if (in && to < kRoom) cand[to] = rank_key(v[q][i], static_cast<uint32_t>(j));
+        n += __popc(who & row_lanes);
       }
     __syncwarp();
-    if (n <= 2 * kWarp) {
-      best = merge_list(0, cand, n, lane);
-    } else {  // a few lanes hold many of the largest: merge the row as it comes
-      for (int j = lane; j < ((r.width + kWarp - 1) & -kWarp); j += kWarp) {
+    const int most = __reduce_max_sync(kFull, n);
+    if (most <= kRoom) {
+      for (int i = 0; i < most; i += kLanes)
+        best = merge_best<kLanes>(best, sort_ascending<kLanes>(i + part < n ? cand[i + part] : 0, lane), lane);
+    } else {  // a few lanes hold many of the largest: merge the rows as they come
+      for (int j = part; j < ((r.width + kLanes - 1) & -kLanes); j += kLanes) {
         const float w = j < r.width && (!kMask || mask[j] != 0) ? to_f32<T>(x[j]) : -kInf;
         const unsigned long long k = w > -kInf ? rank_key(w, static_cast<uint32_t>(j)) : 0;
-        if (__any_sync(kFull, k > __shfl_sync(kFull, best, r.topk - 1)))
-          best = merge_best(best, sort_ascending(k, lane), lane);
+        if (__any_sync(kFull, k > __shfl_sync(kFull, best, lane - part + r.topk - 1)))
+          best = merge_best<kLanes>(best, sort_ascending<kLanes>(k, lane), lane);
       }
     }
   }
-  finish_row<T>(r, o, row, x, mask, targets, target, a, best, lane, kWarp);
+  if (valid) finish_row<T>(r, o, row, x, mask, targets, target, a, best, part, kLanes);
 }
 
 // ---------------------------------------------------------------- wider rows: blocks, joined if several
@@ -763,35 +787,38 @@ __device__ __forceinline__ void slots_grad(const RowView<T>& view, int lo, int h
       });
 }
 
-// A warp per row, for narrow rows with few named columns.
+// kLanes lanes per row, for narrow rows with few named columns.
 constexpr int kNamedNarrow = 64;
-template <typename T, bool kMask>
+template <typename T, bool kMask, int kLanes>
 __global__ void __launch_bounds__(kNarrowThreads) logprob_backward_narrow_kernel(Rows r, const T* __restrict__ logits,
                                                                                  const uint8_t* __restrict__ masks,
                                                                                  Upstream u, T* __restrict__ grads) {
-  __shared__ int sh_id[kNarrowThreads / kWarp][kNamedNarrow];
-  __shared__ float sh_g[kNarrowThreads / kWarp][kNamedNarrow];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kNarrowThreads / kWarp) + warp;
-  if (row >= r.rows) return;
+  constexpr int kRows = kNarrowThreads / kLanes;
+  __shared__ int sh_id[kRows][kNamedNarrow];
+  __shared__ float sh_g[kRows][kNamedNarrow];
+  const int part = threadIdx.x % kLanes, own = threadIdx.x / kLanes;
+  int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + own;
+  if (row - (threadIdx.x & 31) / kLanes >= r.rows) return;  // the whole warp is past the end
+  const bool valid = row < r.rows;
+  row = min(row, r.rows - 1);
   const T* x = logits + row * r.stride;
   const uint8_t* mask = kMask ? masks + row * r.mask_stride : nullptr;
   T* grad = grads + row * r.width;
   float sum = 0.0f;
-  for (int q = lane; q < r.targets + r.topk; q += kWarp) {
+  for (int q = part; q < r.targets + r.topk; q += kLanes) {
     int64_t id;
     const float g = named(r, u, row, q, id);
-    sh_id[warp][q] = static_cast<int>(id);
-    sh_g[warp][q] = g;
+    sh_id[own][q] = static_cast<int>(id);
+    sh_g[own][q] = g;
     sum += g;
   }
-  const RowGrad g = row_grad(r, u, row, warp_sum(sum));
+  const RowGrad g = row_grad(r, u, row, lanes_sum<kLanes>(sum));
   const RowView<T> view(x, mask, r.width);
-  slots_grad<T, kMask, kWarp>(view, 0, view.slots, lane, g, r.c, grad);
+  if (valid) slots_grad<T, kMask, kLanes>(view, 0, view.slots, part, g, r.c, grad);
   __syncwarp();
-  if (!g.none)
-    add_named<T, kMask>(r, g, x, mask, grad, 0, r.width, lane, kWarp, [&](int q) { return sh_id[warp][q]; },
-                        [&](int q) { return sh_g[warp][q]; });
+  if (valid && !g.none)
+    add_named<T, kMask>(r, g, x, mask, grad, 0, r.width, part, kLanes, [&](int q) { return sh_id[own][q]; },
+                        [&](int q) { return sh_g[own][q]; });
 }
 
 template <typename T, bool kMask, int kT>
@@ -896,19 +923,32 @@ template <typename F> int by_type(int32_t dtype, bool mask, F f) {
   }
 }
 
+// Whether narrow rows get eight lanes each: enough of them to fill the SMs that way too (9,000 of 103
+// columns: 10 and 8 us, 8,000 with a warp each: 11 and 11 us; 2,304: 6 us either way), short enough for 16
+// values a lane, and no more alternatives than lanes.
+template <typename T> bool by_eights(const Rows& r) {
+  return r.rows >= 4096 && r.topk <= 8 && (r.width + 2 * kVec<T> - 2) / kVec<T> * kVec<T> <= 128;
+}
+
 template <typename T, bool kMask>
 int launch_narrow(const Rows& r, const void* logits, const uint8_t* mask, const int64_t* targets, const Outputs& o,
                   cudaStream_t st) {
-  constexpr int kRows = kNarrowThreads / kWarp;
-  const unsigned grid = (unsigned)((r.rows + kRows - 1) / kRows);
   const T* x = static_cast<const T*>(logits);
-  const int slots = ((r.width + 2 * kVec<T> - 2) / kVec<T> + kWarp - 1) / kWarp;  // of a lane, at most
-  if (slots <= 1) logprob_narrow_kernel<T, kMask, 1><<<grid, kNarrowThreads, 0, st>>>(r, x, mask, targets, o);
-  else if (slots <= 2) logprob_narrow_kernel<T, kMask, 2><<<grid, kNarrowThreads, 0, st>>>(r, x, mask, targets, o);
-  else if (slots <= 4) logprob_narrow_kernel<T, kMask, 4><<<grid, kNarrowThreads, 0, st>>>(r, x, mask, targets, o);
-  else if (kVec<T> == 8 || slots <= 8)
-    logprob_narrow_kernel<T, kMask, 8><<<grid, kNarrowThreads, 0, st>>>(r, x, mask, targets, o);
-  else logprob_narrow_kernel<T, kMask, 64 / kVec<T>><<<grid, kNarrowThreads, 0, st>>>(r, x, mask, targets, o);
+  const int most = (r.width + 2 * kVec<T> - 2) / kVec<T>;  // slots of a row
+  auto launch = [&](auto slots, auto lanes) {
+    constexpr int kRows = kNarrowThreads / decltype(lanes)::value;
+    logprob_narrow_kernel<T, kMask, decltype(slots)::value, decltype(lanes)::value>
+        <<<(unsigned)((r.rows + kRows - 1) / kRows), kNarrowThreads, 0, st>>>(r, x, mask, targets, o);
+  };
+  using Eight = std::integral_constant<int, 8>;
+  using Warp = std::integral_constant<int, kWarp>;
+  const int per = (most + kWarp - 1) / kWarp;  // of a lane
+  if (by_eights<T>(r)) launch(std::integral_constant<int, 16 / kVec<T>>(), Eight());
+  else if (per <= 1) launch(std::integral_constant<int, 1>(), Warp());
+  else if (per <= 2) launch(std::integral_constant<int, 2>(), Warp());
+  else if (per <= 4) launch(std::integral_constant<int, 4>(), Warp());
+  else if (kVec<T> == 8 || per <= 8) launch(std::integral_constant<int, 8>(), Warp());
+  else launch(std::integral_constant<int, 64 / kVec<T>>(), Warp());
   MKG_LAUNCHED("logprob_narrow_kernel");
   return MKG_OK;
 }
@@ -991,9 +1031,13 @@ int logprob_backward(const mkg_logprob_params* p, const void* logits, const uint
     MKG_REQUIRE(reinterpret_cast<uintptr_t>(x) % sizeof(T) == 0 && reinterpret_cast<uintptr_t>(grad) % sizeof(T) == 0,
                 "logprob_backward: misaligned tensors");
     if (r.width <= kNarrow && r.targets + r.topk <= kNamedNarrow) {
-      constexpr int kRows = kNarrowThreads / kWarp;
-      logprob_backward_narrow_kernel<T, kMask><<<(unsigned)((r.rows + kRows - 1) / kRows), kNarrowThreads, 0, st>>>(
-          r, x, mask, u, static_cast<T*>(grad));
+      auto launch = [&](auto lanes) {
+        constexpr int kRows = kNarrowThreads / decltype(lanes)::value;
+        logprob_backward_narrow_kernel<T, kMask, decltype(lanes)::value>
+            <<<(unsigned)((r.rows + kRows - 1) / kRows), kNarrowThreads, 0, st>>>(r, x, mask, u, static_cast<T*>(grad));
+      };
+      if (by_eights<T>(r)) launch(std::integral_constant<int, 8>());
+      else launch(std::integral_constant<int, kWarp>());
       MKG_LAUNCHED("logprob_backward_narrow_kernel");
       return MKG_OK;
     }

@@ -144,6 +144,20 @@ def test_many_rows():
 
 
 @gpu
+@pytest.mark.parametrize("dtype", (torch.float32, torch.float16))
+@pytest.mark.parametrize("rows, width, topk, mask", ((8192, 103, 5, False), (8197, 25, 8, True), (9001, 122, 1, True),
+                                                     (8200, 7, 8, False), (8193, 1, 3, True), (8192, 123, 9, False)))
+def test_many_narrow_rows(rows, width, topk, mask, dtype):
+    """Enough short rows that several share a warp; the last warps are part full."""
+    x, t, m = case(rows, width, 2, dtype, mask, seed=rows)
+    x[5] = 0.0                      # ties all along
+    x[6, :] = torch.arange(width, device="cuda").to(dtype)
+    out, grad, want = run(x, t, m, 0.9, topk)
+    check(out, want, width)
+    check_grad(grad, want)
+
+
+@gpu
 @pytest.mark.parametrize("width", (40, 1024, 5000, 70001))
 @pytest.mark.parametrize("kind", ("equal", "ascending", "descending", "one thread", "zeros of both signs"))
 def test_ties_and_orders(width, kind):
@@ -157,6 +171,9 @@ def test_ties_and_orders(width, kind):
         out, grad, want = run(x, t, None, 1.0, topk)
         check(out, want, width, f"{kind} top {topk}")
         check_grad(grad, want)
+    if width == 40:  # the same where several rows share a warp
+        out = target_logprobs(x[:1].expand(8192, width), t[:1].expand(8192, 1), topk=7)
+        assert torch.equal(out.top_ids, definition(x[:1], t[:1], 1.0, None, 7)["top_ids"].expand(8192, 7))
 
 
 @gpu
