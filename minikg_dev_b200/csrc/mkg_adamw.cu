@@ -85,14 +85,15 @@ template <> struct Bits<float> { using type = uint4; };
 template <> struct Bits<__nv_bfloat16> { using type = uint2; };
 template <> struct Bits<__half> { using type = uint2; };
 
-template <typename T> __device__ __forceinline__ void spread(const typename Bits<T>::type& raw, float (&out)[kQuad]) {
+template <typename T> __device__ __forceinline__ void spread(typename Bits<T>::type raw, float (&out)[kQuad]) {
   T e[kQuad];
   memcpy(e, &raw, sizeof(raw));
 #pragma unroll
   for (int i = 0; i < kQuad; ++i) out[i] = to_f32<T>(e[i]);
 }
 template <typename T> __device__ __forceinline__ void load_quad(const T* at, float (&out)[kQuad]) {
-  spread<T>(*reinterpret_cast<const typename Bits<T>::type*>(at), out);
+  const typename Bits<T>::type raw = *reinterpret_cast<const typename Bits<T>::type*>(at);
+  spread<T>(raw, out);
 }
 template <typename T> __device__ __forceinline__ void store_quad(T* at, const float (&v)[kQuad]) {
   T e[kQuad];
@@ -161,10 +162,9 @@ __device__ __forceinline__ float to_odd(double x) {
 }
 __device__ __forceinline__ bool finite(double x) { return fabs(x) <= DBL_MAX; }
 
-// smallest e with a <= 1.75 * 2^e
+// smallest e with a <= 1.75 * 2^e: a mantissa above 0.75 carries into the exponent
 __device__ __forceinline__ int exponent_for(float a) {
-  const uint32_t b = __float_as_uint(a);
-  return static_cast<int>(b >> 23) - 127 + ((b & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return static_cast<int>((__float_as_uint(a) + 0x1fffffu) >> 23) - 127;
 }
 __device__ __forceinline__ int first_exponent(float a) { return min(max(exponent_for(a) - 8, kFirstLow), kFirstHigh); }
 __device__ __forceinline__ int second_exponent(float a) { return min(max(exponent_for(a), kSecondLow), kSecondHigh); }
@@ -198,8 +198,14 @@ __device__ __forceinline__ void decode_first(uint32_t w, float scale, float (&ou
   }
 }
 __device__ __forceinline__ void decode_second(uint32_t w, float scale, float (&out)[kQuad]) {
+  if (scale <= 0x1p30f) {
+    const float s = scale * 0x1p96f;
 #pragma unroll
-  for (int i = 0; i < kQuad; ++i) out[i] = __uint_as_float(((w >> (8 * i)) & 255u) << 20) * 0x1p96f * scale;
+    for (int i = 0; i < kQuad; ++i) out[i] = __uint_as_float(((w >> (8 * i)) & 255u) << 20) * s;
+  } else {
+#pragma unroll
+    for (int i = 0; i < kQuad; ++i) out[i] = __uint_as_float(((w >> (8 * i)) & 255u) << 20) * 0x1p96f * scale;
+  }
   if (((w & 0x7f7f7f7fu) + 0x01010101u) & w & 0x80808080u) {  // a byte of 255
 #pragma unroll
     for (int i = 0; i < kQuad; ++i)
@@ -268,7 +274,6 @@ __device__ __forceinline__ void step_held(const Hyper& h, const Held& at, float 
 #pragma unroll
     for (int u = 0; u < kQuads; ++u) {
       uint32_t lo[2], hi[2], t[kQuad];
-      float least = FLT_MAX;
 #pragma unroll
       for (int i = 0; i < kQuad; i += 2) {
         const float d0 = off[u][i] * fi, d1 = off[u][i + 1] * fi, m0 = m[u][i], m1 = m[u][i + 1];
@@ -277,22 +282,26 @@ __device__ __forceinline__ void step_held(const Hyper& h, const Held& at, float 
       }
       const uint32_t low = __byte_perm(lo[0], lo[1], 0x5410);
       fw[u] = __byte_perm(hi[0], hi[1], 0x5410);
-      // the ends differ, and not as 0 and -0
-      again1 |= (nonzero_bytes(low ^ fw[u]) & nonzero_bytes((low | fw[u]) & 0x7f7f7f7fu)) >> u;
+      if (low != fw[u])  // the ends differ, and not as 0 and -0
+        again1 |= (nonzero_bytes(low ^ fw[u]) & nonzero_bytes((low | fw[u]) & 0x7f7f7f7fu)) >> u;
+      uint32_t near = 0xffffffffu;
 #pragma unroll
       for (int i = 0; i < kQuad; ++i) {
         // the code in byte 3, rounded by the byte below it: v32 is off by at most 5 * 2^-24 of itself, 5 units
         // of its last place, and 16 of them around the middle go to fp64
-        const float y = v[u][i] * si * 0x1p-96f;
-        least = fminf(least, y);
-        t[i] = __float_as_uint(y) * 16u + 0x800000u;
-        if (t[i] * 256u + 0x10000u <= 0x20000u) again2 |= 0x80u << (8 * i) >> u;
+        t[i] = __float_as_uint(v[u][i] * si * 0x1p-96f) * 16u + 0x800000u;
+        near = min(near, t[i] * 256u + 0x10000u);
       }
       sw[u] = upper_bytes(t);
-      if (least < 0x1p-129f) {  // below the smallest held value: that one, or 0 where nothing was added up
+      if (near <= 0x20000u) {
 #pragma unroll
         for (int i = 0; i < kQuad; ++i)
-          if (t[i] < 0x1000000u && (v[u][i] > 0.0f || g(u, i) != 0.0f)) sw[u] |= 1u << (8 * i);
+          if (t[i] * 256u + 0x10000u <= 0x20000u) again2 |= 0x80u << (8 * i) >> u;
+      }
+      if (nonzero_bytes(sw[u]) != 0x80808080u) {  // below the smallest held value: that, or 0 where nothing was added up
+#pragma unroll
+        for (int i = 0; i < kQuad; ++i)
+          if (((sw[u] >> (8 * i)) & 255u) == 0 && (v[u][i] > 0.0f || g(u, i) != 0.0f)) sw[u] |= 1u << (8 * i);
       }
     }
   } else {  // the block's largest values, exactly
