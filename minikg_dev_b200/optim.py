@@ -34,6 +34,9 @@ class _Plan:
         table = ctypes.c_int64 * len(self.numel)
         self.tables = tuple(table(*v) for v in (self.numel, self.offset, self.index))
 
+    def __reduce__(self):  # ctypes arrays do not pickle
+        return _Plan, (self.numel, self.offset, self.index)
+
     def part(self, at) -> "_Plan":
         return _Plan(*([v[i] for i in at] for v in (self.numel, self.offset, self.index)))
 
@@ -45,7 +48,8 @@ class AdamW(torch.optim.Optimizer):
 
     ``lr`` is a number or a float32 CUDA tensor of one element; a captured step reads the tensor
     at every replay, a number is kept as it was at capture.  Parameters without a gradient are left
-    alone and their step count with them.  Not offered: sparse or complex gradients, ``amsgrad``,
+    alone and their step count with them.  A step can be captured after ``load_kernels()`` or a first step;
+    gradients must then stay where they are (``zero_grad(set_to_none=False)``).  Not offered: sparse or complex gradients, ``amsgrad``,
     ``maximize``; non-contiguous parameters and parameters that share memory are refused.  Two steps
     of one optimizer must not run at the same time.
     """
@@ -93,7 +97,7 @@ class AdamW(torch.optim.Optimizer):
             if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
                 raise ValueError("AdamW: parameters share memory")
             if isinstance(group["lr"], torch.Tensor) and every and group["lr"].device != every[0].device:
-                raise ValueError("AdamW: a tensor lr must be one float32 value on the parameters' device")
+                raise ValueError(f"AdamW: a tensor lr must be on {every[0].device}, got {group['lr'].device}")
         except Exception:
             del self.param_groups[before:]
             raise
@@ -187,6 +191,8 @@ class AdamW(torch.optim.Optimizer):
         self._check_group(group)
         dev, lr = self._buffers["steps"].device, group["lr"]
         on_device = isinstance(lr, torch.Tensor)
+        if on_device and lr.device != dev:
+            raise ValueError(f"AdamW: a tensor lr must be on {dev}, got {lr.device}")
         b1, b2 = group["betas"]
         hyper = N.AdamwParams(0.0 if on_device else float(lr), float(b1), float(b2), float(group["eps"]),
                               float(group["weight_decay"]), lr.data_ptr() if on_device else None, N.DTYPES[p_dtype],
@@ -249,6 +255,9 @@ class AdamW(torch.optim.Optimizer):
                 merged["lr"] = have["lr"]  # a captured step reads this tensor
             merged["betas"] = tuple(merged["betas"])
             self._check_group(merged)
+            if new.get("amsgrad") or new.get("maximize") or (new.get("decoupled_weight_decay") is False
+                                                             and merged["weight_decay"]):
+                raise ValueError("AdamW: the state dict is of an optimizer with amsgrad, maximize or coupled decay")
         if not self._buffers:
             return
         entries = []
@@ -259,9 +268,8 @@ class AdamW(torch.optim.Optimizer):
                     continue
                 if "exp_avg" not in e and _CODES[0] not in e:
                     raise ValueError("AdamW: a state dict entry without moments")
-                if "exp_avg" in e and bool((e["exp_avg_sq"] < 0).any()):
-                    raise ValueError("AdamW: a state dict entry with negative second moments")
-                if e["exp_avg" if "exp_avg" in e else _CODES[0]].numel() != n:
+                names = ("exp_avg", "exp_avg_sq") if "exp_avg" in e else (_CODES[0], _CODES[2])
+                if any(e[k].numel() != n for k in names):
                     raise ValueError("AdamW: a state dict entry of another size")
                 entries.append((e, n, at, i))
         dev = self._buffers["steps"].device
@@ -287,6 +295,8 @@ class AdamW(torch.optim.Optimizer):
             if "exp_avg" in e:
                 m[at:at + n].copy_(e["exp_avg"].reshape(-1))
                 v[at:at + n].copy_(e["exp_avg_sq"].reshape(-1))
+        if bool((v < 0).any()):
+            raise ValueError("AdamW: a state dict entry with negative second moments")
         self._buffers["steps"].copy_(steps)
         if self.state_bits == 32:
             self._buffers["exp_avg"][:self._total].copy_(m[:self._total])

@@ -329,8 +329,24 @@ def test_state_dicts(start, bits):
     copied.param_groups[0]["params"][0].grad = twins[0].grad.clone()
     copied.step()
     assert int(copied.state[copied.param_groups[0]["params"][0]]["step"]) == int(dst.state[twins[0]]["step"]) + 1
+    import pickle
+    again = pickle.loads(pickle.dumps(dst))
+    for q, r in zip(twins, again.param_groups[0]["params"]):
+        r.grad = q.grad.clone()
+    dst.step()
+    again.step()
+    for q, r in zip(twins, again.param_groups[0]["params"]):
+        assert torch.equal(q, r)
     with pytest.raises(ValueError, match="groups"):
         AdamW(twins[:2]).load_state_dict(saved)
+    for change in (dict(amsgrad=True), dict(maximize=True), dict(decoupled_weight_decay=False)):
+        with pytest.raises(ValueError, match="amsgrad"):
+            dst.load_state_dict({**saved, "param_groups": [{**saved["param_groups"][0], **change}]})
+    key = next(iter(saved["state"]))
+    if "exp_avg_sq" in saved["state"][key]:
+        saved["state"][key]["exp_avg_sq"] = -saved["state"][key]["exp_avg_sq"]
+        with pytest.raises(ValueError, match="negative"):
+            dst.load_state_dict(saved)
 
 
 @gpu
