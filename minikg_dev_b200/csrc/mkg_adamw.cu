@@ -367,6 +367,15 @@ template <bool kPlain> __device__ __forceinline__ float quotient(float m, float 
   return __fdividef(m, fmaf(root, r, eps));
 }
 
+// b^n by squaring, off by about n units of 2^-53 of itself, which 1 - b^n does not see once b^n is small.  A
+// block waits for it: pow and a division in fp64 kept the first chunk of each waiting for several us.
+__device__ __forceinline__ double power(double b, int64_t n) {
+  double r = 1.0;
+  for (; n > 0; n >>= 1, b *= b)
+    if (n & 1) r *= b;
+  return r;
+}
+
 template <int kCap> __device__ __forceinline__ int tensor_of(const Table<kCap>& t, int chunk) {
   int lo = 0, hi = t.n - 1;  // the last tensor whose first chunk is not after this one
   while (lo < hi) {
@@ -395,15 +404,13 @@ __global__ void __launch_bounds__(kThreads, k8 ? kBlocks8 : kBlocks32) adamw_ker
       known = e;
       turn ^= 1;
       if (tid < 2) {  // the other warps need them only after their moments; the last ones may still be in use
-        const double n = static_cast<double>(s.steps[t.index[e]] + 1);
         const double lr = h.lr_device ? static_cast<double>(*h.lr_device) : h.lr;
-        const double left = 1.0 - pow(tid == 0 ? h.beta1 : h.beta2, n);
-        const double q = (tid == 0 ? lr : 1.0) / (tid == 0 ? left : sqrt(left));
+        const float left = static_cast<float>(1.0 - power(tid == 0 ? h.beta1 : h.beta2, s.steps[t.index[e]] + 1));
         if (tid == 0) {
           sh_rates[turn].decay = static_cast<float>(1.0 - lr * h.weight_decay);
-          sh_rates[turn].step = static_cast<float>(q);
+          sh_rates[turn].step = static_cast<float>(lr) / left;
         } else {
-          sh_rates[turn].root = static_cast<float>(q);
+          sh_rates[turn].root = 1.0f / sqrtf(left);
         }
       }
       __syncwarp();
