@@ -106,8 +106,7 @@ template <typename T> __device__ __forceinline__ void store_quad(T* at, const fl
 }
 // A lane's share of a whole block as it is in memory, moments in 8 bits: what a warp loads for its next
 // block while it works on this one.
-template <typename P, typename G> struct Share {
-  typename Bits<P>::type p[kQuads];
+template <typename G> struct Share {  // the parameters, needed last, are loaded when the block's turn comes
   typename Bits<G>::type g[kQuads];
   uint32_t first[kQuads], second[kQuads];
   float first_scale, second_scale;
@@ -301,7 +300,7 @@ __device__ __forceinline__ void step_held(const Hyper& h, const Held& at, float 
       if (nonzero_bytes(sw[u]) != 0x80808080u) {  // below the smallest held value: that, or 0 where nothing was added up
 #pragma unroll
         for (int i = 0; i < kQuad; ++i)
-          if (((sw[u] >> (8 * i)) & 255u) == 0 && (v[u][i] > 0.0f || g(u, i) != 0.0f)) sw[u] |= 1u << (8 * i);
+          if (((sw[u] >> (8 * i)) & 255u) == 0 && (v[u][i] > 0.0f || again(u * kQuad + i) != 0.0f)) sw[u] |= 1u << (8 * i);
       }
     }
   } else {  // the block's largest values, exactly
@@ -315,8 +314,9 @@ __device__ __forceinline__ void step_held(const Hyper& h, const Held& at, float 
       decode_second(at.second[u * kWarp], ss, ov);
 #pragma unroll
       for (int i = 0; i < kQuad; ++i) {
-        high1 = fmaxf(high1, magnitude(first_sum(h, om[i], g(u, i))));
-        high2 = fmaxf(high2, magnitude(second_sum(h, ov[i], g(u, i))));
+        const float gi = again(u * kQuad + i);
+        high1 = fmaxf(high1, magnitude(first_sum(h, om[i], gi)));
+        high2 = fmaxf(high2, magnitude(second_sum(h, ov[i], gi)));
       }
     }
     fe = first_exponent(warp_max(high1));
@@ -394,7 +394,7 @@ __global__ void __launch_bounds__(kThreads, k8 ? kBlocks8 : kBlocks32) adamw_ker
   const int chunks = t.chunk[t.n];
   int known = -1, turn = 0;
   const bool plain = h.eps >= 0x1p-60f;
-  Share<P, G> next;    // moments in 8 bits
+  Share<G> next;    // moments in 8 bits
   bool ready = false;  // next holds the block that comes
   const int end = min((static_cast<int>(blockIdx.x) + 1) * run, chunks);
   for (int chunk = blockIdx.x * run; chunk < end; ++chunk) {
@@ -433,7 +433,6 @@ __global__ void __launch_bounds__(kThreads, k8 ? kBlocks8 : kBlocks32) adamw_ker
 #pragma unroll
           for (int u = 0; u < kQuads; ++u) {
             const int64_t j = ahead * kBlock + (u * kWarp + lane) * kQuad;
-            next.p[u] = *reinterpret_cast<const typename Bits<P>::type*>(p + j);
             next.g[u] = *reinterpret_cast<const typename Bits<G>::type*>(g + j);
             next.first[u] = first[ahead * (kBlock / kQuad) + u * kWarp];
             next.second[u] = second[ahead * (kBlock / kQuad) + u * kWarp];
@@ -442,12 +441,12 @@ __global__ void __launch_bounds__(kThreads, k8 ? kBlocks8 : kBlocks32) adamw_ker
           next.second_scale = s.second_scale[block + ahead];
         };
         if (whole) {
+          load_block(p, left, true, lane, pv);
           if (!ready) fetch(0);
           fs = next.first_scale;
           ss = next.second_scale;
 #pragma unroll
           for (int u = 0; u < kQuads; ++u) {
-            spread<P>(next.p[u], pv[u]);
             spread<G>(next.g[u], gv[u]);
             decode_first(next.first[u], fs, mv[u]);
             decode_second(next.second[u], ss, vv[u]);

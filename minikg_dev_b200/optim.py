@@ -22,7 +22,7 @@ import torch
 
 from . import _native as N
 
-_dtype, _layout = attrgetter("dtype"), attrgetter("layout")
+_dtype, _layout, _grad = attrgetter("dtype"), attrgetter("layout"), attrgetter("grad")
 _CODES = ("exp_avg_codes", "exp_avg_scale", "exp_avg_sq_codes", "exp_avg_sq_scale")
 
 
@@ -163,15 +163,16 @@ class AdamW(torch.optim.Optimizer):
             params = group["params"]
             if len(params) != len(plan.numel):
                 raise RuntimeError("AdamW: a group's parameters changed after it was added")
-            grads = [p.grad for p in params]
-            if any(g is None for g in grads):
+            grads = list(map(_grad, params))
+            if type(None) in set(map(type, grads)):
                 at = [i for i, g in enumerate(grads) if g is not None]
                 params, grads, plan = [params[i] for i in at], [grads[i] for i in at], plan.part(at)
-            kinds = set(zip(map(_dtype, params), map(_dtype, grads)))
-            if len(kinds) == 1:
+            if not grads:
+                continue
+            if len(set(map(_dtype, params))) == 1 and len(set(map(_dtype, grads))) == 1:
                 self._launch(group, params, grads, plan)
                 continue
-            for kind in sorted(kinds, key=str):
+            for kind in sorted(set(zip(map(_dtype, params), map(_dtype, grads))), key=str):
                 at = [i for i, (p, g) in enumerate(zip(params, grads)) if (p.dtype, g.dtype) == kind]
                 self._launch(group, [params[i] for i in at], [grads[i] for i in at], plan.part(at))
         return loss
