@@ -371,6 +371,24 @@ def test_streams_and_graphs():
     assert torch.equal(grad, want_grad)
 
 
+@gpu
+def test_two_streams_at_once():
+    """Calls in flight together share nothing: each has its own workspace."""
+    cases = [case(3, 300007, 2, torch.float32, False, seed=20 + i)[:2] for i in range(4)]
+    want = [target_logprobs(x, t, 1.0, None, 12) for x, t in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(5):
+        for s, (x, t) in zip(streams, cases):
+            with torch.cuda.stream(s):
+                got.append(target_logprobs(x, t, 1.0, None, 12))
+    torch.cuda.synchronize()
+    for i, out in enumerate(got):
+        for a, b in zip(out, want[i % 4]):
+            assert torch.equal(a, b)
+
+
 # ------------------------------------------------------------------------------ refusals (CPU)
 @pytest.mark.parametrize("change, error", [
     (dict(logits=torch.zeros(2, 5, dtype=torch.float64)), TypeError),
