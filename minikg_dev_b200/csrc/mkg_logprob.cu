@@ -30,6 +30,7 @@ constexpr int kTopMax = MKG_LOGPROB_TOPK_MAX;
 constexpr int kResident = 1024, kResidentTop = 1536;
 constexpr int kNarrowThreads = 64;   // two rows, a warp each
 constexpr int64_t kNarrow = 2040;    // rows up to this width are held by one warp: 64 values a lane, wherever they start
+constexpr int64_t kManyRows = 4096;  // enough to fill the SMs with a warp or a block each
 constexpr int kCand = 256;           // alternatives collected before they are ordered
 constexpr int64_t kWidthMax = int64_t(1) << 30;
 constexpr unsigned kFull = 0xffffffffu;
@@ -334,6 +335,29 @@ template <int kLanes> __device__ __forceinline__ float lanes_sum(float v) {
   return v;
 }
 
+// The kLanes largest keys of each row of a warp, descending over its lanes, from its n candidates in shared
+// memory; more than fit (a few lanes hold many of the largest): from the row itself, merged as it comes.
+template <typename T, bool kMask, int kLanes>
+__device__ __forceinline__ unsigned long long order_lanes(const unsigned long long* cand, int n, int room,
+                                                          const Rows& r, const T* x, const uint8_t* mask, int lane,
+                                                          int part) {
+  __syncwarp();
+  unsigned long long best = 0;
+  const int most = __reduce_max_sync(kFull, n);
+  if (most <= room) {
+    for (int i = 0; i < most; i += kLanes)
+      best = merge_best<kLanes>(best, sort_ascending<kLanes>(i + part < n ? cand[i + part] : 0, lane), lane);
+  } else {
+    for (int j = part; j < ((r.width + kLanes - 1) & -kLanes); j += kLanes) {
+      const float w = j < r.width && (!kMask || mask[j] != 0) ? to_f32<T>(x[j]) : -kInf;
+      const unsigned long long k = w > -kInf ? rank_key(w, static_cast<uint32_t>(j)) : 0;
+      if (__any_sync(kFull, k > __shfl_sync(kFull, best, lane - part + r.topk - 1)))
+        best = merge_best<kLanes>(best, sort_ascending<kLanes>(k, lane), lane);
+    }
+  }
+  return best;
+}
+
 template <typename T, bool kMask, int kSlots, int kLanes>
 __global__ void __launch_bounds__(kNarrowThreads) logprob_narrow_kernel(Rows r, const T* __restrict__ logits,
                                                                         const uint8_t* __restrict__ masks,
@@ -406,19 +430,7 @@ __global__ void __launch_bounds__(kNarrowThreads) logprob_narrow_kernel(Rows r, 
         if (in && to < kRoom) cand[to] = rank_key(v[q][i], static_cast<uint32_t>(j));
         n += __popc(who & row_lanes);
       }
-    __syncwarp();
-    const int most = __reduce_max_sync(kFull, n);
-    if (most <= kRoom) {
-      for (int i = 0; i < most; i += kLanes)
-        best = merge_best<kLanes>(best, sort_ascending<kLanes>(i + part < n ? cand[i + part] : 0, lane), lane);
-    } else {  // a few lanes hold many of the largest: merge the rows as they come
-      for (int j = part; j < ((r.width + kLanes - 1) & -kLanes); j += kLanes) {
-        const float w = j < r.width && (!kMask || mask[j] != 0) ? to_f32<T>(x[j]) : -kInf;
-        const unsigned long long k = w > -kInf ? rank_key(w, static_cast<uint32_t>(j)) : 0;
-        if (__any_sync(kFull, k > __shfl_sync(kFull, best, lane - part + r.topk - 1)))
-          best = merge_best<kLanes>(best, sort_ascending<kLanes>(k, lane), lane);
-      }
-    }
+    best = order_lanes<T, kMask, kLanes>(cand, n, kRoom, r, x, mask, lane, part);
   }
   if (valid) finish_row<T>(r, o, row, x, mask, targets, target, a, best, part, kLanes);
 }
@@ -480,6 +492,107 @@ template <typename T> __device__ __forceinline__ void consume(const float (&v)[k
   }
 }
 
+// A thread's slots of [lo, hi), kT apart: its moments, and the key of its largest element and the slot where
+// that was first met (0: no candidate).
+template <typename T, bool kMask, int kT>
+__device__ __forceinline__ unsigned long long stream_slots(const RowView<T>& view, int lo, int hi, int tid, float c,
+                                                           Moments& a) {
+  Stream own{-kInf, -kInf, -kInf, 0, 0, 0};
+  for_slots<T, kT>(
+      view, lo, hi, tid,
+      [&](int slot, int n, auto full) {
+        typename RowView<T>::Raw raw[kUnroll];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u)
+          if (full || u < n) raw[u] = view.template fetch<kMask>(slot + u * kT);
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+          if (!full && u >= n) break;
+          float v[kVec<T>];
+          view.template values<kMask>(raw[u], v);
+          consume<T>(v, slot + u * kT, c, own);
+        }
+      },
+      [&](int slot) {
+        float v[kVec<T>];
+        view.template load<kMask>(slot, v);
+        consume<T>(v, slot, c, own);
+      });
+  float s0, s1, t0, t1;
+  unpack2(own.s, s0, s1);
+  unpack2(own.t, t0, t1);
+  a = {own.ref, s0 + s1, t0 + t1};
+  shift_to(a, own.m, c);
+  a.m = own.m;
+  return a.m > -kInf ? rank_key(a.m, static_cast<uint32_t>(own.at)) : 0;
+}
+
+// Many rows that a warp streams each, or eight lanes: no registers hold the row, so 32 to 40 warps an SM hide
+// the loads, and nothing waits at a barrier.  Alternatives as in a block: the best lanes' slots again (from L1 or
+// L2).
+constexpr int kStreamThreads = 128;
+template <typename T, bool kMask, int kLanes>
+__global__ void __launch_bounds__(kStreamThreads, kMask ? 8 : 10)
+    logprob_stream_kernel(Rows r, const T* __restrict__ logits, const uint8_t* __restrict__ masks,
+                          const int64_t* __restrict__ targets, Outputs o) {
+  constexpr int kRows = kStreamThreads / kLanes, kRoom = 2 * kLanes;
+  __shared__ unsigned long long sh_cand[kRows][kRoom];
+  __shared__ int sh_winner[kRows][kLanes];
+  const int lane = threadIdx.x & 31, part = lane % kLanes, own = threadIdx.x / kLanes;
+  int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + own;
+  if (row - lane / kLanes >= r.rows) return;  // the whole warp is past the end
+  const bool valid = row < r.rows;  // others of the warp repeat the last row and write nothing
+  row = min(row, r.rows - 1);
+  const T* x = logits + row * r.stride;
+  const uint8_t* mask = kMask ? masks + row * r.mask_stride : nullptr;
+  const RowView<T> view(x, mask, r.width);
+  const Target target = read_target<T>(r, targets, row, part, x, mask);
+  Moments a;
+  const unsigned long long mine = stream_slots<T, kMask, kLanes>(view, 0, view.slots, part, r.c, a);
+  const float M = lanes_max<kLanes>(a.m);
+  shift_to(a, M, r.c);
+  a = {M, lanes_sum<kLanes>(a.s), lanes_sum<kLanes>(a.t)};
+  unsigned long long best = 0;
+  if (r.topk > 0) {
+    const unsigned long long sorted = sort_ascending<kLanes>(mine, lane);
+    const unsigned long long floor = __shfl_sync(kFull, sorted, lane - part + kLanes - r.topk);
+    const float least = floor ? packed_value(floor) : -kInf;
+    const uint32_t least_slot = floor ? packed_rank(floor) : 0xffffffffu;
+    const unsigned before = ((1u << part) - 1) << (lane - part);  // the row's lanes before this one
+    const unsigned row_lanes = (kLanes == kWarp ? kFull : (1u << (kLanes & 31)) - 1) << (lane - part);
+    const bool winner = mine != 0 && mine >= floor;
+    const unsigned winners = __ballot_sync(kFull, winner) & row_lanes;
+    if (winner) sh_winner[own][__popc(winners & before)] = part;
+    __syncwarp();
+    const int per = (view.slots + kLanes - 1) / kLanes;  // slots of a lane
+    const int pairs = __popc(winners) * per;
+    const int most_pairs = __reduce_max_sync(kFull, pairs);
+    unsigned long long* cand = sh_cand[own];
+    int n = 0;
+    for (int q = part; q < ((most_pairs + kLanes - 1) & -kLanes); q += kLanes) {
+      const int slot = q < pairs ? sh_winner[own][q / per] + q % per * kLanes : view.slots;
+      float v[kVec<T>];
+      if (slot < view.slots) {
+        view.template load<kMask>(slot, v);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kVec<T>; ++i) v[i] = -kInf;
+      }
+#pragma unroll
+      for (int i = 0; i < kVec<T>; ++i) {
+        const bool in = v[i] > least || (v[i] == least && v[i] > -kInf && static_cast<uint32_t>(slot) <= least_slot);
+        const unsigned who = __ballot_sync(kFull, in);
+        if (who == 0) continue;
+        const int to = n + __popc(who & before);
+        if (in && to < kRoom) cand[to] = rank_key(v[i], static_cast<uint32_t>(view.first(slot) + i));
+        n += __popc(who & row_lanes);
+      }
+    }
+    best = order_lanes<T, kMask, kLanes>(cand, n, kRoom, r, x, mask, lane, part);
+  }
+  if (valid) finish_row<T>(r, o, row, x, mask, targets, target, a, best, part, kLanes);
+}
+
 template <typename T, bool kMask, bool kTop, int kT>
 __global__ void __launch_bounds__(kT, (kTop && !kMask ? kResidentTop : kResident) / kT)
     logprob_wide_kernel(Rows r, const T* __restrict__ logits, const uint8_t* __restrict__ masks,
@@ -502,34 +615,8 @@ __global__ void __launch_bounds__(kT, (kTop && !kMask ? kResidentTop : kResident
   if (splits > 1) cudaTriggerProgrammaticLaunchCompletion();  // the joining kernel may come and wait
   else target = read_target<T>(r, targets, row, tid, x, mask);
 
-  Stream own{-kInf, -kInf, -kInf, 0, 0, 0};
-  for_slots<T, kT>(
-      view, lo, hi, tid,
-      [&](int slot, int n, auto full) {
-        typename RowView<T>::Raw raw[kUnroll];
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u)
-          if (full || u < n) raw[u] = view.template fetch<kMask>(slot + u * kT);
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-          if (!full && u >= n) break;
-          float v[kVec<T>];
-          view.template values<kMask>(raw[u], v);
-          consume<T>(v, slot + u * kT, r.c, own);
-        }
-      },
-      [&](int slot) {
-        float v[kVec<T>];
-        view.template load<kMask>(slot, v);
-        consume<T>(v, slot, r.c, own);
-      });
-  float s0, s1, t0, t1;
-  unpack2(own.s, s0, s1);
-  unpack2(own.t, t0, t1);
-  Moments a{own.ref, s0 + s1, t0 + t1};
-  shift_to(a, own.m, r.c);
-  a.m = own.m;
-  const unsigned long long mine = a.m > -kInf ? rank_key(a.m, static_cast<uint32_t>(own.at)) : 0;
+  Moments a;
+  const unsigned long long mine = stream_slots<T, kMask, kT>(view, lo, hi, tid, r.c, a);
   const Moments all = block_join<kWarps>(a, r.c, sh_m);
 
   unsigned long long best = 0;
@@ -901,8 +988,8 @@ Cut in_pieces(int64_t slots, int64_t piece, int threads) {
 constexpr int64_t kForwardPiece = 4096, kBackwardPiece = 2048;
 Cut forward_cut(const mkg_logprob_params* p) {
   const int64_t slots = most_slots(p);
-  // enough rows to go round: 4,096 blocks need no joining (5 to 8 us with its launch)
-  if (p->rows >= 4096) return in_pieces(slots, slots, 128);
+  // enough rows to go round: they need no joining (5 to 8 us with its launch)
+  if (p->rows >= kManyRows) return in_pieces(slots, slots, 128);
   // about one row per SM: larger blocks instead of several and a join (256 x 17,050: 14 us, 30 us)
   if (p->rows >= 128 && p->rows < 512 && slots < 8192) return in_pieces(slots, slots, 512);
   const int64_t even = slots * p->rows / persistent_blocks(4);  // few rows: smaller pieces, to reach every SM
@@ -923,12 +1010,21 @@ template <typename F> int by_type(int32_t dtype, bool mask, F f) {
   }
 }
 
-// Whether narrow rows get eight lanes each: enough of them to fill the SMs that way too (9,000 of 103
-// columns: 10 and 8 us, 8,000 with a warp each: 11 and 11 us; 2,304: 6 us either way), short enough for 16
-// values a lane, and no more alternatives than lanes.
-template <typename T> bool by_eights(const Rows& r) {
-  return r.rows >= 4096 && r.topk <= 8 && (r.width + 2 * kVec<T> - 2) / kVec<T> * kVec<T> <= 128;
+constexpr int64_t kEightsWide = 512;
+template <typename T> bool fits_eights(const Rows& r) {  // 16 values a lane
+  return r.topk <= 8 && (r.width + 2 * kVec<T> - 2) / kVec<T> * kVec<T> <= 128;
 }
+// Whether a warp streams each row.  65,536 rows of 1,645 fp32 logits: 102 us that way and 102 us held in
+// registers, but 146 and 261 us with a mask, 161 and 265 us with 8 alternatives, and bf16 96 and 170 us.  20,000
+// rows of 7,275: 115 us, and 129 us with a block each (bf16 79 and 127 us); with alternatives topk of the 32 lanes
+// are read again, and past about 5 KB of a row that costs more than a block's ordering (8 of fp32: 185 and 148 us,
+// of bf16: 121 and 165 us).
+bool streams(const Rows& r, int64_t size) {
+  const int64_t bytes = r.width * size;
+  return r.rows >= kManyRows && r.width > kEightsWide && (r.topk == 0 ? bytes <= 65536 : bytes * r.topk <= 32 * 5120);
+}
+bool by_lanes(const Rows& r, int64_t size) { return r.width <= kNarrow || streams(r, size); }
+int64_t size_of(int32_t dtype) { return dtype == MKG_F32 ? 4 : 2; }
 
 template <typename T, bool kMask>
 int launch_narrow(const Rows& r, const void* logits, const uint8_t* mask, const int64_t* targets, const Outputs& o,
@@ -943,7 +1039,15 @@ int launch_narrow(const Rows& r, const void* logits, const uint8_t* mask, const 
   using Eight = std::integral_constant<int, 8>;
   using Warp = std::integral_constant<int, kWarp>;
   const int per = (most + kWarp - 1) / kWarp;  // of a lane
-  if (by_eights<T>(r)) launch(std::integral_constant<int, 16 / kVec<T>>(), Eight());
+  auto stream = [&](auto lanes) {
+    constexpr int kRows = kStreamThreads / decltype(lanes)::value;
+    logprob_stream_kernel<T, kMask, decltype(lanes)::value>
+        <<<(unsigned)((r.rows + kRows - 1) / kRows), kStreamThreads, 0, st>>>(r, x, mask, targets, o);
+  };
+  const bool many = r.rows >= kManyRows;
+  if (many && fits_eights<T>(r)) launch(std::integral_constant<int, 16 / kVec<T>>(), Eight());
+  else if (many && r.topk == 0 && r.width <= kEightsWide) stream(Eight());
+  else if (streams(r, sizeof(T))) stream(Warp());
   else if (per <= 1) launch(std::integral_constant<int, 1>(), Warp());
   else if (per <= 2) launch(std::integral_constant<int, 2>(), Warp());
   else if (per <= 4) launch(std::integral_constant<int, 4>(), Warp());
@@ -957,7 +1061,7 @@ int launch_narrow(const Rows& r, const void* logits, const uint8_t* mask, const 
 
 size_t logprob_workspace_bytes(const mkg_logprob_params* p) {
   Rows r;
-  if (check_params(p, &r) != MKG_OK || p->width <= kNarrow) return 0;
+  if (check_params(p, &r) != MKG_OK || by_lanes(r, size_of(p->dtype))) return 0;
   const Cut cut = forward_cut(p);
   if (cut.splits == 1) return 0;
   return (size_t)(p->rows * cut.splits) * (sizeof(Partial) + (size_t)p->topk * sizeof(unsigned long long));
@@ -982,7 +1086,7 @@ int logprob_forward(const mkg_logprob_params* p, const void* logits, const uint8
     constexpr bool kMask = decltype(has_mask)::value;
     const T* x = static_cast<const T*>(logits);
     MKG_REQUIRE(reinterpret_cast<uintptr_t>(x) % sizeof(T) == 0, "logprob_forward: misaligned logits");
-    if (p->width <= kNarrow) return launch_narrow<T, kMask>(r, logits, mask, targets, o, st);
+    if (by_lanes(r, sizeof(T))) return launch_narrow<T, kMask>(r, logits, mask, targets, o, st);
     const Cut cut = forward_cut(p);
     MKG_REQUIRE(r.rows * cut.splits < (int64_t(1) << 31), "logprob_forward: too many rows");
     Partial* partials = static_cast<Partial*>(ws);
@@ -1036,7 +1140,7 @@ int logprob_backward(const mkg_logprob_params* p, const void* logits, const uint
         logprob_backward_narrow_kernel<T, kMask, decltype(lanes)::value>
             <<<(unsigned)((r.rows + kRows - 1) / kRows), kNarrowThreads, 0, st>>>(r, x, mask, u, static_cast<T*>(grad));
       };
-      if (by_eights<T>(r)) launch(std::integral_constant<int, 8>());
+      if (r.rows >= kManyRows && r.width <= kEightsWide) launch(std::integral_constant<int, 8>());
       else launch(std::integral_constant<int, kWarp>());
       MKG_LAUNCHED("logprob_backward_narrow_kernel");
       return MKG_OK;

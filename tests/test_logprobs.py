@@ -372,6 +372,32 @@ def test_streams_and_graphs():
 
 
 @gpu
+@pytest.mark.parametrize("dtype", (torch.float32, torch.bfloat16))
+@pytest.mark.parametrize("rows, width, topk, mask", ((4096, 300, 0, False), (4099, 513, 5, True), (4101, 1201, 20, False),
+                                                     (4097, 2600, 8, True), (4096, 5003, 0, True), (4100, 130, 0, True),
+                                                     (4098, 1500, 32, True)))
+def test_many_streamed_rows(rows, width, topk, mask, dtype):
+    """Enough rows of middling length that a warp, or eight lanes, stream each."""
+    x, t, m = case(rows, width, 2, dtype, mask, seed=rows + width)
+    x[5] = 0.0                      # ties all along
+    x[6, :] = torch.arange(width, device="cuda").to(dtype)
+    x[7, :] = torch.where(torch.arange(width, device="cuda") // 4 % 32 == 3, 9.0, 0.0).to(dtype)  # one lane has them all
+    x[8, 1] = math.nan
+    if m is not None:
+        m[8, 1] = False             # off the candidates: not seen
+    else:
+        x[8, 1] = 0.0
+    out, grad, want = run(x, t, m, 0.9, topk)
+    check(out, want, width)
+    check_grad(grad, want)
+    x[9, width - 1] = math.inf
+    if m is not None:
+        m[9, width - 1] = True
+    bad = target_logprobs(x, t, 0.9, m, topk)
+    assert torch.isnan(bad.lse[9]) and (bad.top_ids[9] == -1).all() and torch.equal(bad.top_ids[:9], out.top_ids[:9])
+
+
+@gpu
 def test_two_streams_at_once():
     """Calls in flight together share nothing: each has its own workspace."""
     cases = [case(3, 300007, 2, torch.float32, False, seed=20 + i)[:2] for i in range(4)]
