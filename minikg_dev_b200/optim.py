@@ -243,6 +243,14 @@ class AdamW(torch.optim.Optimizer):
                                               N.stream_handle(dev)), "adamw_unpack")
         return m[:self._total], v[:self._total]
 
+    def state_dict(self):
+        """``torch.optim.Optimizer.state_dict`` with the step counts as ``torch.optim.AdamW`` has them (float32
+        on the host), which continues from moments in 32 bits."""
+        out = super().state_dict()
+        steps = self._buffers["steps"].tolist() if self._buffers else []
+        out["state"] = {k: {**e, "step": torch.tensor(float(steps[k]))} for k, e in out["state"].items()}
+        return out
+
     def load_state_dict(self, state_dict) -> None:
         """Loads a state dict of this class or of ``torch.optim.AdamW`` into the buffers in place: moments
         given as fp32 values are rounded to what 8 bits hold, moments given in 8 bits are read as the

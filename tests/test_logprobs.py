@@ -186,7 +186,10 @@ def test_strides_and_masks(width):
     wide_mask = torch.rand(6, width + 5, generator=g, device="cuda") < 0.5
     for x in (big[:, 3:3 + width], big[:, 1:1 + width], big[::2, :width], big[:1, 5:5 + width].expand(6, width),
               torch.randn(width, 6, generator=g, device="cuda").t()):
-        for m in (None, row_mask, wide_mask[:x.shape[0], 2:2 + width], row_mask[None].expand(x.shape[0], width)):
+        across = torch.zeros(width, x.shape[0], dtype=torch.bool, device="cuda")
+        across[::3] = True
+        for m in (None, row_mask, wide_mask[:x.shape[0], 2:2 + width], row_mask[None].expand(x.shape[0], width),
+                  across.t()):
             out, grad, want = run(x, t[:x.shape[0]], m, 1.0, 6)
             check(out, want, width)
             check_grad(grad, want)
@@ -369,6 +372,19 @@ def test_streams_and_graphs():
     want_grad, = torch.autograd.grad(o.logprobs, fresh, static)
     assert torch.equal(out.logprobs, o.logprobs) and torch.equal(out.top_ids, o.top_ids)
     assert torch.equal(grad, want_grad)
+
+
+@gpu
+@pytest.mark.parametrize("rows, width", ((3, 40), (4, 2500), (2, 70001), (4100, 600)))
+def test_many_targets(rows, width):
+    """More targets than lanes, threads or columns: each column collects all that is named there."""
+    s = 1024 if rows < 100 else 70
+    x, t, m = case(rows, width, s, torch.float32, True, seed=width)
+    t[1, 5:] = t[1, 5]  # one column, over and over
+    t[2 % rows, ::2] = -1
+    out, grad, want = run(x, t, m, 1.1, 3)
+    check(out, want, width)
+    check_grad(grad, want)
 
 
 @gpu

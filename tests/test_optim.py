@@ -350,6 +350,24 @@ def test_state_dicts(start, bits):
 
 
 @gpu
+def test_torch_takes_the_state():
+    """A state dict with moments in 32 bits continues in torch.optim.AdamW."""
+    pairs = make((700, (3, 5)), torch.float32, torch.float32, seed=9)
+    a = AdamW([p for p, _ in pairs], lr=0.02)
+    for _ in range(3):
+        a.step()
+    twins = [torch.nn.Parameter(p.detach().clone()) for p, _ in pairs]
+    b = torch.optim.AdamW(twins, lr=0.5)
+    b.load_state_dict(copy.deepcopy(a.state_dict()))
+    for q, (_, g) in zip(twins, pairs):
+        q.grad = g.clone()
+    a.step()
+    b.step()
+    for (p, _), q in zip(pairs, twins):
+        assert float((p - q).abs().max()) <= 16 * U * 0.02 * 4 + 4 * U * float(q.abs().max())
+
+
+@gpu
 @pytest.mark.parametrize("bits", (32, 8))
 def test_captured_steps(bits):
     """A captured step replayed is the step itself, with the rate read from its tensor."""
