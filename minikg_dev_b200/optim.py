@@ -26,6 +26,16 @@ _dtype, _layout, _grad = attrgetter("dtype"), attrgetter("layout"), attrgetter("
 _CODES = ("exp_avg_codes", "exp_avg_scale", "exp_avg_sq_codes", "exp_avg_sq_scale")
 
 
+def _run(buffer, at, n):
+    """``buffer[at:at + n]`` of a flat buffer, in one operation."""
+    return torch.as_strided(buffer, (n,), (1,), at)
+
+
+def _blocks(at, n):
+    """The blocks of scales of ``n`` moments that start at ``at``: (first, how many)."""
+    return at // N.ADAMW_BLOCK, -(-n // N.ADAMW_BLOCK)
+
+
 class _Plan:
     """Sizes, offsets into the flat moments and step-count indexes of a group's parameters."""
 
@@ -131,16 +141,15 @@ class AdamW(torch.optim.Optimizer):
     def _views(self) -> None:
         """``state[p]``: each parameter's part of the flat buffers."""
         b = self._buffers
+        steps = b["steps"].unbind()
         for group, plan in zip(self.param_groups, self._plan):
             for p, n, at, i in zip(group["params"], plan.numel, plan.offset, plan.index):
+                m, v = (torch.as_strided(b[k], p.shape, p.stride(), at) for k in ("exp_avg", "exp_avg_sq"))
                 if self.state_bits == 32:
-                    moments = {k: b[k][at:at + n].view(p.shape) for k in ("exp_avg", "exp_avg_sq")}
+                    self.state[p] = {"step": steps[i], "exp_avg": m, "exp_avg_sq": v}
                 else:
-                    blocks = slice(at // N.ADAMW_BLOCK, -(-(at + n) // N.ADAMW_BLOCK))
-                    moments = dict(zip(_CODES, (b["exp_avg"][at:at + n].view(p.shape), b["exp_avg_scale"][blocks],
-                                                b["exp_avg_sq"][at:at + n].view(p.shape),
-                                                b["exp_avg_sq_scale"][blocks])))
-                self.state[p] = {"step": b["steps"][i], **moments}
+                    sm, sv = (_run(b[k], *_blocks(at, n)) for k in ("exp_avg_scale", "exp_avg_sq_scale"))
+                    self.state[p] = {"step": steps[i], **dict(zip(_CODES, (m, sm, v, sv)))}
 
     def _state_struct(self, buffers=None) -> N.AdamwState:
         b = buffers or self._buffers
@@ -286,24 +295,23 @@ class AdamW(torch.optim.Optimizer):
         codes = {k: torch.zeros(max(self._total, 1), dtype=torch.uint8, device=dev) for k in ("exp_avg", "exp_avg_sq")}
         codes |= {k: torch.zeros(max(self._total // N.ADAMW_BLOCK, 1), device=dev) for k in _CODES[1::2]}
         codes |= {k: self._buffers[k] for k in ("steps", "ticket")}
-        any_codes = False
-        for e, n, at, _ in entries:
-            if "exp_avg" in e:
-                continue
-            any_codes = True
-            blocks = slice(at // N.ADAMW_BLOCK, -(-(at + n) // N.ADAMW_BLOCK))
-            codes["exp_avg"][at:at + n].copy_(e[_CODES[0]].reshape(-1))
-            codes["exp_avg_scale"][blocks].copy_(e[_CODES[1]])
-            codes["exp_avg_sq"][at:at + n].copy_(e[_CODES[2]].reshape(-1))
-            codes["exp_avg_sq_scale"][blocks].copy_(e[_CODES[3]])
-        if any_codes:
+        coded = [x for x in entries if "exp_avg" not in x[0]]
+        for e, n, at, _ in coded:
+            blocks = _blocks(at, n)
+            for buffer, name, run in zip(("exp_avg", "exp_avg_scale", "exp_avg_sq", "exp_avg_sq_scale"), _CODES,
+                                         ((at, n), blocks, (at, n), blocks)):
+                _run(codes[buffer], *run).copy_(e[name].reshape(-1))
+        if coded:
             m, v = (x.contiguous() for x in self._unpacked(codes))
-        steps = torch.zeros(max(self._tensors, 1), dtype=torch.int64)
+        counts = [0] * max(self._tensors, 1)
         for e, n, at, i in entries:
-            steps[i] = int(e["step"])
-            if "exp_avg" in e:
-                m[at:at + n].copy_(e["exp_avg"].reshape(-1))
-                v[at:at + n].copy_(e["exp_avg_sq"].reshape(-1))
+            counts[i] = int(e["step"])
+        steps = torch.tensor(counts, dtype=torch.int64)
+        plain = [x for x in entries if "exp_avg" in x[0]]
+        for buffer, name in ((m, "exp_avg"), (v, "exp_avg_sq")):
+            if plain:
+                torch._foreach_copy_([_run(buffer, at, n) for _, n, at, _ in plain],
+                                     [e[name].detach().reshape(-1) for e, *_ in plain])
         if bool((v < 0).any()):
             raise ValueError("AdamW: a state dict entry with negative second moments")
         self._buffers["steps"].copy_(steps)

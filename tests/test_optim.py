@@ -350,6 +350,29 @@ def test_state_dicts(start, bits):
 
 
 @gpu
+@pytest.mark.parametrize("bits", (32, 8))
+@pytest.mark.parametrize("where, dtype", (("cpu", torch.float32), ("cuda", torch.float64), ("cuda", torch.bfloat16)))
+def test_state_from_elsewhere(bits, where, dtype):
+    """Moments on the host, of other types, not contiguous, beside empty parameters and missing entries."""
+    params = [torch.nn.Parameter(torch.randn(s, device="cuda")) for s in ((0,), (30, 9), (256,), (1, 1), (4, 0))]
+    opt = AdamW(params, state_bits=bits)
+    wide = [torch.randn(9, 30, device=where).to(dtype).t(), torch.ones(1, 1, device=where, dtype=dtype)]
+    saved = opt.state_dict()
+    saved["state"] = {k: {"step": 7.0, "exp_avg": x, "exp_avg_sq": x.abs()} for k, x in zip((1, 3), wide)}
+    saved["state"][4] = {"step": torch.tensor(2), "exp_avg": params[4].data, "exp_avg_sq": params[4].data}
+    opt.load_state_dict(saved)
+    m, v = opt.moments()
+    for at, x in ((0, wide[0]), (768, wide[1]), (512, torch.zeros(256))):
+        x = x.float().cpu().reshape(-1)
+        want = (x, x.abs()) if bits == 32 else held(x, x.abs())
+        got = m[at:at + x.numel()].cpu(), v[at:at + x.numel()].cpu()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b.float())
+    assert [int(opt.state[p]["step"]) for p in params] == [0, 7, 0, 7, 2]
+    assert all(t.shape == p.shape for p in params for k, t in opt.state[p].items() if k in ("exp_avg", "exp_avg_codes"))
+
+
+@gpu
 def test_torch_takes_the_state():
     """A state dict with moments in 32 bits continues in torch.optim.AdamW."""
     pairs = make((700, (3, 5)), torch.float32, torch.float32, seed=9)
