@@ -14,6 +14,7 @@ from pathlib import Path
 import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libminikg_b200.so"
+TENSORS_LIB_PATH = LIB_PATH.with_name("libminikg_tensors.so")
 
 MKG_OK = 0
 MASK_NONE, MASK_U8, MASK_F32 = 0, 1, 2
@@ -216,6 +217,23 @@ def load(path: Path | str | None = None):
             fn.argtypes = args
         _lib = lib
         return lib
+
+
+_gather = None
+
+
+def gather_gradients():
+    """``mkg_gather_gradients`` of ``_lib/libminikg_tensors.so``, which reads a list of torch tensors
+    under the interpreter's lock; raises if it was not built."""
+    global _gather
+    if _gather is None:
+        if not TENSORS_LIB_PATH.exists():
+            raise RuntimeError(f"minikg_b200 native library missing at {TENSORS_LIB_PATH}; run "
+                               "`python -m minikg_dev_b200.build`")
+        fn = C.PyDLL(str(TENSORS_LIB_PATH)).mkg_gather_gradients
+        fn.restype, fn.argtypes = i64, [C.py_object, i64, i64, vp, vp, vp, vp, vp]
+        _gather = fn
+    return _gather
 
 
 def exported_symbols() -> list[str]:

@@ -3,7 +3,8 @@
     python -m minikg_dev_b200.build [--verbose-ptxas] [--force]
 
 Each ``csrc/*.cu`` compiles to an object under ``_build/`` (skipped when newer than its
-sources), then one shared library links them.  No JIT cache is involved: the ``.so``
+sources), then one shared library links them.  ``csrc/mkg_tensors.cpp``, which reads lists of torch
+tensors, becomes ``_lib/libminikg_tensors.so`` with g++ against the installed torch.  No JIT cache is involved: the ``.so``
 lives next to the package so it travels with the source tree.
 """
 from __future__ import annotations
@@ -13,6 +14,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -23,6 +25,8 @@ INCLUDE = ROOT / "include"
 BUILD = ROOT / "_build"
 LIB_DIR = PKG / "_lib"
 LIB = LIB_DIR / "libminikg_b200.so"
+TENSORS = CSRC / "mkg_tensors.cpp"
+TENSORS_LIB = LIB_DIR / "libminikg_tensors.so"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
@@ -62,6 +66,18 @@ def _compile(src: Path, verbose_ptxas: bool) -> tuple[Path, str]:
     return obj, res.stderr
 
 
+def _build_tensors() -> None:
+    import torch
+    root = Path(torch.__file__).resolve().parent
+    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-shared",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", f"-I{sysconfig.get_paths()['include']}",
+           *(f"-isystem{root / d}" for d in ("include", "include/torch/csrc/api/include")), str(TENSORS),
+           "-o", str(TENSORS_LIB), f"-L{root / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed on {TENSORS.name}:\n{res.stderr}\n{res.stdout}")
+
+
 def build(force: bool = False, verbose_ptxas: bool = False, quiet: bool = True) -> Path:
     BUILD.mkdir(exist_ok=True)
     LIB_DIR.mkdir(exist_ok=True)
@@ -69,6 +85,8 @@ def build(force: bool = False, verbose_ptxas: bool = False, quiet: bool = True) 
     hdrs = headers()
     todo = [s for s in srcs if force or verbose_ptxas or _stale(BUILD / (s.stem + ".o"), [s, *hdrs])]
     logs = []
+    if force or _stale(TENSORS_LIB, [TENSORS]):
+        _build_tensors()
     if todo:
         with ThreadPoolExecutor(max_workers=min(8, len(todo))) as ex:
             for obj, log in ex.map(lambda s: _compile(s, verbose_ptxas), todo):

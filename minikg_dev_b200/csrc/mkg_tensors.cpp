@@ -1,0 +1,76 @@
+// What an optimizer step asks of its tensors, for a whole list in one call.
+//
+// A step over many small parameters is bound by the host: a question to one tensor costs about 50 ns from
+// Python (its type, layout, size, device, address; twice, for the gradient too), which for 131 tensors
+// is 110 us before a launch of 15 us.  Asked here it is a few nanoseconds each.  Nothing is kept between calls.
+#include <torch/csrc/autograd/python_variable.h>
+
+#include <cstdint>
+
+namespace {
+
+enum Status : int64_t {
+    kFine = 0,
+    kOther = 1,     // something that is not a tensor
+    kDense = 2,     // a gradient that is not dense
+    kLayout = 3,    // a parameter or gradient of another size or layout than when it was added
+    kDevice = 4,    // on another device
+    kType = 5,      // of another type
+    kFailed = 6,    // a C++ exception
+};
+
+int type_of(const at::Tensor& t) {  // MKG_F32, MKG_BF16, MKG_F16
+    switch (t.scalar_type()) {
+        case at::kFloat: return 0;
+        case at::kBFloat16: return 1;
+        case at::kHalf: return 2;
+        default: return -1;
+    }
+}
+
+bool on(const at::Tensor& t, int64_t device) {
+    return t.is_cuda() && t.get_device() == device;
+}
+
+}  // namespace
+
+// params: a list of n tensors.  For each with a gradient: their addresses and kinds[i] = (type of the
+// parameter) + 4 (type of the gradient) + 16 if the gradient has to be made contiguous first (its address
+// is not given then); -1 without a gradient.  Returns the status, at[0] the index it is of; at[1] tells
+// whether all kinds are the same.  Called with the interpreter's lock.
+extern "C" __attribute__((visibility("default"))) int64_t mkg_gather_gradients(PyObject* params, int64_t n,
+                                                                              int64_t device, const int64_t* numel,
+                                                                              int64_t* p_at, int64_t* g_at,
+                                                                              int32_t* kinds, int64_t* at) {
+    at[0] = 0;
+    at[1] = 1;
+    if (!PyList_Check(params) || PyList_GET_SIZE(params) != n) return kOther;
+    try {
+        for (int64_t i = 0; i < n; ++i) {
+            at[0] = i;
+            PyObject* o = PyList_GET_ITEM(params, i);
+            if (!THPVariable_Check(o)) return kOther;
+            const at::Tensor& p = THPVariable_Unpack(o);
+            const at::Tensor g = p.grad();
+            kinds[i] = -1;
+            p_at[i] = g_at[i] = 0;
+            if (g.defined()) {
+                const int pt = type_of(p), gt = type_of(g);
+                if (pt < 0 || gt < 0) return kType;
+                if (g.layout() != at::kStrided) return kDense;
+                if (p.layout() != at::kStrided || p.numel() != numel[i] || g.numel() != numel[i] ||
+                    !p.is_contiguous() || p.is_neg())
+                    return kLayout;
+                if (!on(p, device) || !on(g, device)) return kDevice;
+                const bool plain = g.is_contiguous() && !g.is_neg();
+                kinds[i] = pt + 4 * gt + (plain ? 0 : 16);
+                p_at[i] = reinterpret_cast<int64_t>(p.mutable_data_ptr());
+                if (plain) g_at[i] = reinterpret_cast<int64_t>(g.const_data_ptr());
+            }
+            if (kinds[i] != kinds[0]) at[1] = 0;
+        }
+    } catch (...) {
+        return kFailed;
+    }
+    return kFine;
+}

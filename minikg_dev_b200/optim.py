@@ -16,13 +16,12 @@ from __future__ import annotations
 import ctypes
 import math
 from itertools import accumulate
-from operator import attrgetter
 
 import torch
 
 from . import _native as N
 
-_dtype, _layout, _grad = attrgetter("dtype"), attrgetter("layout"), attrgetter("grad")
+_TYPES = list(N.DTYPES)  # by their numbers
 _CODES = ("exp_avg_codes", "exp_avg_scale", "exp_avg_sq_codes", "exp_avg_sq_scale")
 
 
@@ -46,9 +45,6 @@ class _Plan:
 
     def __reduce__(self):  # ctypes arrays do not pickle
         return _Plan, (self.numel, self.offset, self.index)
-
-    def part(self, at) -> "_Plan":
-        return _Plan(*([v[i] for i in at] for v in (self.numel, self.offset, self.index)))
 
 
 class AdamW(torch.optim.Optimizer):
@@ -172,18 +168,8 @@ class AdamW(torch.optim.Optimizer):
             params = group["params"]
             if len(params) != len(plan.numel):
                 raise RuntimeError("AdamW: a group's parameters changed after it was added")
-            grads = list(map(_grad, params))
-            if type(None) in set(map(type, grads)):
-                at = [i for i, g in enumerate(grads) if g is not None]
-                params, grads, plan = [params[i] for i in at], [grads[i] for i in at], plan.part(at)
-            if not grads:
-                continue
-            if len(set(map(_dtype, params))) == 1 and len(set(map(_dtype, grads))) == 1:
-                self._launch(group, params, grads, plan)
-                continue
-            for kind in sorted(set(zip(map(_dtype, params), map(_dtype, grads))), key=str):
-                at = [i for i, (p, g) in enumerate(zip(params, grads)) if (p.dtype, g.dtype) == kind]
-                self._launch(group, [params[i] for i in at], [grads[i] for i in at], plan.part(at))
+            if params:
+                self._launch(group, params, plan)
         return loss
 
     def load_kernels(self) -> None:
@@ -211,27 +197,42 @@ class AdamW(torch.optim.Optimizer):
             N.check(N.load().mkg_adamw_step(hyper, self._state_struct(), len(numel), p_at, g_at, numel, offset, index,
                                             N.stream_handle(dev)), "adamw_step")
 
-    def _launch(self, group, params, grads, plan) -> None:
-        dev = self._buffers["steps"].device
-        n, dtypes = len(params), (params[0].dtype, grads[0].dtype)
-        if dtypes[0] not in N.DTYPES or dtypes[1] not in N.DTYPES:
-            raise TypeError(f"AdamW: parameters of {dtypes[0]} with gradients of {dtypes[1]}")
-        if set(map(_layout, grads)) != {torch.strided}:
-            raise RuntimeError("AdamW: gradients must be dense")
-        if not all(map(torch.Tensor.is_contiguous, grads)):
-            grads = [g.detach().contiguous() for g in grads]
-        if (list(map(torch.Tensor.numel, params)) != plan.numel or list(map(torch.Tensor.numel, grads)) != plan.numel
-                or not all(map(torch.Tensor.is_contiguous, params))):
-            raise RuntimeError("AdamW: a parameter changed its size or layout, or its gradient has another size")
-        where = set(map(torch.Tensor.get_device, params))
-        where.update(map(torch.Tensor.get_device, grads))
-        if where != {dev.index}:
-            raise RuntimeError(f"AdamW: parameters and gradients must be on {dev}")
+    def _launch(self, group, params, plan) -> None:
+        dev, n = self._buffers["steps"].device, len(params)
         table = ctypes.c_int64 * n
-        p_at = table(*map(torch.Tensor.data_ptr, params))
-        g_at = table(*map(torch.Tensor.data_ptr, grads))
-        self._call(group, *dtypes, p_at, g_at, *plan.tables)
-        torch.autograd.graph.increment_version(params)
+        p_at, g_at, kinds, at = table(), table(), (ctypes.c_int32 * n)(), (ctypes.c_int64 * 2)()
+        status = N.gather_gradients()(params, n, dev.index, plan.tables[0], p_at, g_at, kinds, at)
+        if status:
+            raise self._refusal(status, params[at[0]], dev)
+        held = []  # contiguous copies of gradients, until the launch
+        if at[1] and 0 <= kinds[0] < 16:
+            parts = ((kinds[0], None),)
+        else:
+            every = list(kinds)
+            for i, k in enumerate(every):
+                if k >= 16:
+                    held.append(params[i].grad.detach().resolve_neg().contiguous())
+                    every[i], g_at[i] = k - 16, held[-1].data_ptr()
+            parts = [(k, [i for i, other in enumerate(every) if other == k]) for k in sorted(set(every) - {-1})]
+        for kind, only in parts:
+            tables, updated = (p_at, g_at, *plan.tables), params
+            if only is not None and len(only) < n:
+                short = ctypes.c_int64 * len(only)
+                tables, updated = [short(*(t[i] for i in only)) for t in tables], [params[i] for i in only]
+            self._call(group, _TYPES[kind % 4], _TYPES[kind // 4], *tables)
+            torch.autograd.graph.increment_version(updated)
+
+    @staticmethod
+    def _refusal(status, p, dev) -> Exception:
+        if status == 2:
+            return RuntimeError("AdamW: gradients must be dense")
+        if status == 3:
+            return RuntimeError("AdamW: a parameter changed its size or layout, or its gradient has another size")
+        if status == 4:
+            return RuntimeError(f"AdamW: parameters and gradients must be on {dev}")
+        if status == 5:
+            return TypeError(f"AdamW: parameters of {p.dtype} with gradients of {p.grad.dtype}")
+        return RuntimeError("AdamW: a parameter or gradient without memory of its own")
 
     # ------------------------------------------------------------------ the moments
     def moments(self) -> tuple[torch.Tensor, torch.Tensor]:

@@ -488,6 +488,70 @@ def test_refusals_on_the_cpu():
         AdamW([torch.nn.Parameter(torch.ones(5, 6).t())])
 
 
+def test_gathering_on_the_cpu():
+    """The list of tensors that a step reads: what it refuses, and which entry it is of."""
+    import ctypes
+
+    from minikg_dev_b200.build import build
+    build()
+
+    def gather(params, numel=None, device=0):
+        n = len(numel or params)
+        table = ctypes.c_int64 * n
+        sizes = table(*(numel or [p.numel() for p in params]))
+        p_at, g_at, kinds, at = table(), table(), (ctypes.c_int32 * n)(), (ctypes.c_int64 * 2)()
+        status = N.gather_gradients()(params, n, device, sizes, p_at, g_at, kinds, at)
+        return status, at[0], at[1], list(kinds)
+
+    def parameter(grad=True, shape=(3, 4), dtype=torch.float32):
+        p = torch.nn.Parameter(torch.ones(shape, dtype=dtype))
+        if grad:
+            p.grad = torch.ones_like(p)
+        return p
+
+    assert gather([parameter(False), parameter(False)]) == (0, 1, 1, [-1, -1])
+    assert gather([]) == (0, 0, 1, [])
+    assert gather([parameter(False), parameter()])[:2] == (4, 1)  # on the host
+    assert gather([parameter(False), None], [12, 12])[:2] == (1, 1)
+    assert gather([parameter(), parameter()], [12])[0] == 1  # another length
+    assert gather((parameter(),))[0] == 1  # not a list
+    assert gather([parameter(False), parameter(), parameter()], [12, 13, 12])[:2] == (3, 1)
+    assert gather([parameter(False), parameter(dtype=torch.float64)])[:2] == (5, 1)
+    sparse, turned = parameter(), parameter()
+    sparse.grad = torch.ones(3, 4).to_sparse()
+    turned.data = torch.ones(4, 3).t()
+    assert gather([parameter(False), sparse])[:2] == (2, 1)
+    assert gather([turned])[:2] == (3, 0)
+
+
+@gpu
+def test_gradients_of_every_kind():
+    """Missing, transposed, broadcast and lazily negated gradients and two types in one group."""
+    g = torch.Generator(device="cuda").manual_seed(5)
+    shapes = ((6, 5), (300, 4), (7,), (4, 4), (2, 3), (1,), (9, 2))
+    params = [torch.nn.Parameter(torch.randn(s, generator=g, device="cuda")) for s in shapes]
+    params.append(torch.nn.Parameter(torch.randn(40, generator=g, device="cuda").bfloat16()))
+    params[0].grad = torch.randn(5, 6, generator=g, device="cuda").t()
+    params[1].grad = torch.randn(4, generator=g, device="cuda").expand(300, 4)
+    params[2].grad = torch._neg_view(torch.randn(7, generator=g, device="cuda"))
+    params[4].grad = torch.randn(2, 3, generator=g, device="cuda")
+    params[7].grad = torch.randn(40, generator=g, device="cuda").bfloat16()
+    twins = [torch.nn.Parameter(p.detach().clone()) for p in params]
+    for p, q in zip(params, twins):
+        if p.grad is not None:
+            q.grad = p.grad.resolve_neg().contiguous().clone()
+    versions = [p._version for p in params]
+    a, b = AdamW(params, lr=0.1), [AdamW([q], lr=0.1) for q in twins if q.grad is not None]
+    for _ in range(2):
+        a.step()
+        for o in b:
+            o.step()
+    for i, (p, q) in enumerate(zip(params, twins)):
+        assert torch.equal(p, q), i
+        assert int(a.state[p]["step"]) == (0 if p.grad is None else 2)
+        assert (p._version > versions[i]) == (p.grad is not None)
+
+
 @gpu
 def test_refusals():
     flat = torch.ones(100, device="cuda")
