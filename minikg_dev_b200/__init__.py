@@ -13,6 +13,6 @@ Public surface:
 * ``graph``: device CSR build and ``DeviceGraph``;
 * ``synth``: seeded synthetic knowledge graphs of the benchmark shapes.
 The CUDA code lives in ``csrc/`` and is built into ``_lib/libminikg_b200.so`` by
-``python -m minikg_dev_b200.build``.
+``python -m minikg_dev_b200.build``, which also makes ``_lib/libminikg_tensors.so`` for ``optim``.
 """
 __version__ = "0.1.0"
