@@ -52,6 +52,10 @@ class AdamW(torch.optim.Optimizer):
     contiguous CUDA parameters (float32, bfloat16 or float16; gradients in any of the three), all on
     one device.  Arithmetic is fp32 and each parameter is rounded to its type once.
 
+    Gradients of another type than their parameter's: a 16-bit parameter whose ``grad_dtype`` is torch's default
+    gets ``grad_dtype = None`` here, so a program may give it a gradient in 32 bits (autograd's own stay in
+    its type); for a float32 parameter the program sets it.
+
     ``lr`` is a number or a float32 CUDA tensor of one element; a captured step reads the tensor
     at every replay, a number is kept as it was at capture.  Parameters without a gradient are left
     alone and their step count with them.  A step can be captured after ``load_kernels()`` or a first step;
@@ -108,6 +112,15 @@ class AdamW(torch.optim.Optimizer):
             del self.param_groups[before:]
             raise
         self._extend(group["params"])
+        self._open_gradients(group["params"])
+
+    @staticmethod
+    def _open_gradients(params) -> None:
+        """16-bit parameters may have gradients of any type; a type that the program has set stays.  float32 ones
+        are left alone: torch would no longer widen 16-bit gradients before it adds them up."""
+        for p in params:
+            if p.dtype != torch.float32 and p.grad_dtype == p.dtype:
+                p.grad_dtype = None
 
     def _extend(self, params) -> None:
         """Room in the flat buffers for one more group; a graph captured before has to be captured again."""
@@ -155,6 +168,11 @@ class AdamW(torch.optim.Optimizer):
 
     def __getstate__(self):
         return self.__dict__.copy()
+
+    def __setstate__(self, state) -> None:
+        super().__setstate__(state)
+        for group in self.param_groups:
+            self._open_gradients(group["params"])
 
     # ------------------------------------------------------------------ the step
     def step(self, closure=None):

@@ -631,3 +631,33 @@ def test_struct_layouts(tmp_path):
         got = [int(v) for v in subprocess.run([str(tmp_path / "layout")], capture_output=True, text=True,
                                               check=True).stdout.split()]
         assert got == [getattr(cls, f).offset for f in fields] + [ctypes.sizeof(cls)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float16))
+def test_sixteen_bit_parameters_take_gradients_in_32_bits(dtype):
+    """A gradient in 32 bits can be given to them as it is, after copying and unpickling too; a type that
+    the program has chosen stays, and so does the type of a gradient that autograd brings."""
+    import pickle
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    p = torch.nn.Parameter(torch.randn(300, generator=gen, device="cuda").to(dtype))
+    g = torch.randn(300, generator=gen, device="cuda")
+    opt = AdamW([p])
+    p.grad = g
+    before, zero = p.detach().clone(), torch.zeros_like(g)
+    opt.step()
+    want, *_ = definition(before, g, zero, zero, 1)
+    close(p, want, (torch.finfo(dtype).eps / 2 + 32 * U) * (want.abs() + 2e-3), "32-bit gradient")
+    for again in (copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
+        q = again.param_groups[0]["params"][0]
+        q.grad = g
+        again.step()
+    opt.step()
+    assert torch.equal(p, q)
+    p.grad = None
+    (p * 2).sum().backward()
+    assert p.grad.dtype == dtype
+    chosen, wide = (torch.nn.Parameter(torch.ones(4, device="cuda", dtype=t)) for t in (dtype, torch.float32))
+    chosen.grad_dtype = torch.float32
+    AdamW([chosen, wide])
+    assert chosen.grad_dtype is torch.float32 and wide.grad_dtype is torch.float32
