@@ -146,7 +146,6 @@ def prepare(case, seed):
                 i: {"step": case["step"], "exp_avg": s["m"][at:at + n].view(shape),
                     "exp_avg_sq": s["v"][at:at + n].view(shape)} for i, (at, shape, n) in enumerate(spans)}})
         for p, (at, shape, n) in zip(params, spans):
-            p.grad_dtype = DTYPES[case["grad"]]
             p.grad = s["grad"][at:at + n].view(shape)
         s["opt"] = opt
         s["m"] = s["v"] = None
