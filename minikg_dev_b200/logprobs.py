@@ -63,15 +63,21 @@ def _as_rows(t: torch.Tensor | None):
     return t, stride
 
 
-def _forward(logits, targets, mask, tau: float, topk: int, stats):
-    """(parameters, logprobs, entropy, lse, top_ids, top_logprobs); targets int64, contiguous; ``stats``
-    (fp32 [..., 2] or None) receives what the backward needs."""
-    lib, dev, lead = N.load(), logits.device, logits.shape[:-1]
+def _reading(logits, targets, mask, tau: float, topk: int):
+    """(parameters, logits, mask) of one call of the library: both tensors as it reads them, with their strides."""
     x, stride = _as_rows(logits)
     m, m_stride = _as_rows(mask)
-    rows = math.prod(lead)
-    p = N.LogprobParams(rows, logits.shape[-1], stride, m_stride, targets.shape[-1] if targets.dim() > len(lead) else 1,
-                        topk, tau, N.DTYPES[logits.dtype], 0)
+    p = N.LogprobParams(math.prod(logits.shape[:-1]), logits.shape[-1], stride, m_stride,
+                        targets.shape[-1] if targets.dim() == logits.dim() else 1, topk, tau, N.DTYPES[logits.dtype], 0)
+    return p, x, m
+
+
+def _forward(logits, targets, mask, tau: float, topk: int, stats):
+    """(logprobs, entropy, lse, top_ids, top_logprobs); targets int64, contiguous; ``stats`` (fp32 [..., 2] or
+    None) receives what the backward needs."""
+    lib, dev, lead = N.load(), logits.device, logits.shape[:-1]
+    p, x, m = _reading(logits, targets, mask, tau, topk)
+    rows = p.rows
     if stats is None:  # nobody differentiates: one allocation, the outputs are its parts
         s, k = targets.numel(), rows * topk
         buffer = torch.empty(s + 2 * rows + k, dtype=torch.float32, device=dev)
@@ -90,15 +96,21 @@ def _forward(logits, targets, mask, tau: float, topk: int, stats):
                                         entropy.data_ptr(), lse.data_ptr(), top_ids.data_ptr(),
                                         top_logprobs.data_ptr(), N.ptr(stats), N.ptr(ws), need,
                                         N.error_word(dev).data_ptr(), N.stream_handle(dev)), "logprob_forward")
-    return p, logprobs, entropy, lse, top_ids, top_logprobs
+    return logprobs, entropy, lse, top_ids, top_logprobs
+
+
+def _kind(t: torch.Tensor | None):
+    return None if t is None else (t.shape, t.dtype, t.device)
 
 
 class _TargetLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, mask, tau: float, topk: int):
         stats = torch.empty((*logits.shape[:-1], 2), dtype=torch.float32, device=logits.device)
-        ctx.p, logprobs, entropy, lse, top_ids, top_logprobs = _forward(logits, targets, mask, tau, topk, stats)
-        ctx.save_for_backward(logits, targets, mask, top_ids, entropy, stats)
+        logprobs, entropy, lse, top_ids, top_logprobs = _forward(logits, targets, mask, tau, topk, stats)
+        saved = logits, targets, mask, top_ids, entropy, stats
+        ctx.save_for_backward(*saved)
+        ctx.call, ctx.kinds = (tau, topk), tuple(map(_kind, saved))
         ctx.mark_non_differentiable(top_ids)
         ctx.set_materialize_grads(False)
         return logprobs, entropy, lse, top_ids, top_logprobs
@@ -106,14 +118,18 @@ class _TargetLogprobs(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, g_logprobs, g_entropy, g_lse, _g_ids, g_top):
-        logits, targets, mask, top_ids, entropy, stats = ctx.saved_tensors
+        saved = ctx.saved_tensors
+        # hooks on saved tensors (checkpointing, offloading) may hand back copies with other strides
+        if tuple(map(_kind, saved)) != ctx.kinds:
+            raise RuntimeError("target_logprobs: a saved tensor came back with another shape, type or device")
+        logits, _, mask = saved[:3]
+        targets, top_ids, entropy, stats = (t.contiguous() for t in (saved[1], *saved[3:]))
+        p, x, m = _reading(logits, targets, mask, *ctx.call)
         dev = logits.device
-        x, _ = _as_rows(logits)
-        m, _ = _as_rows(mask)
         ups = [g if g is None or g.is_contiguous() else g.contiguous() for g in (g_logprobs, g_entropy, g_lse, g_top)]
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
         with N.on_device(dev):
-            N.check(N.load().mkg_logprob_backward(ctx.p, x.data_ptr(), N.ptr(m), targets.data_ptr(),
+            N.check(N.load().mkg_logprob_backward(p, x.data_ptr(), N.ptr(m), targets.data_ptr(),
                                                   top_ids.data_ptr(), entropy.data_ptr(), stats.data_ptr(),
                                                   *map(N.ptr, ups), grad.data_ptr(), N.stream_handle(dev)),
                     "logprob_backward")
@@ -167,4 +183,4 @@ def target_logprobs(logits: torch.Tensor, targets: torch.Tensor, tau: float = 1.
     m = None if mask is None else mask.view(torch.uint8)
     if logits.requires_grad and torch.is_grad_enabled():
         return TargetLogprobs(*_TargetLogprobs.apply(logits, t, m, tau, int(topk)))
-    return TargetLogprobs(*_forward(logits, t, m, tau, int(topk), None)[1:])
+    return TargetLogprobs(*_forward(logits, t, m, tau, int(topk), None))

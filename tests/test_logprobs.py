@@ -491,3 +491,91 @@ def test_params_layout(tmp_path):
     got = [int(v) for v in subprocess.run([str(tmp_path / "layout")], capture_output=True, text=True,
                                           check=True).stdout.split()]
     assert got == [getattr(N.LogprobParams, f).offset for f in fields] + [ctypes.sizeof(N.LogprobParams)]
+
+
+class Recorder:
+    """Stands in for the library on the host: remembers what it was asked to read."""
+
+    def __init__(self):
+        self.calls = []
+
+    def mkg_logprob_workspace_bytes(self, p):
+        return 0
+
+    def _note(self, p, x, m):
+        self.calls.append((p.rows, p.width, p.row_stride, p.mask_row_stride, x, m))
+        return 0
+
+    def mkg_logprob_forward(self, p, x, m, *rest):
+        return self._note(p, x, m)
+
+    def mkg_logprob_backward(self, p, x, m, *rest):
+        return self._note(p, x, m)
+
+
+def test_the_backward_reads_what_saved_tensor_hooks_hand_back(monkeypatch):
+    """Its strides are those of the tensors that arrive: hooks that pack a copy return a slice as a contiguous
+    tensor.  Tensors of another type or shape are refused."""
+    import contextlib
+
+    from minikg_dev_b200 import logprobs as L
+    lib = Recorder()
+    monkeypatch.setattr(N, "load", lambda: lib)
+    monkeypatch.setattr(N, "on_device", lambda d: contextlib.nullcontext())
+    monkeypatch.setattr(N, "stream_handle", lambda d=None: 0)
+    monkeypatch.setattr(N, "error_word", lambda d: torch.zeros(1, dtype=torch.int32))
+    x = torch.randn(6, 128)[:, :100].detach().requires_grad_(True)
+    m = (torch.rand(6, 160) < 0.5)[:, 20:120].view(torch.uint8)
+    t = torch.zeros(6, 2, dtype=torch.int64)
+    arrived = []
+
+    def unpack(v):
+        arrived.append(v)
+        return v
+
+    def packed(copy):
+        lib.calls.clear()
+        arrived.clear()
+        with torch.autograd.graph.saved_tensors_hooks(copy, unpack):
+            out = L._TargetLogprobs.apply(x, t, m, 1.0, 3)
+        out[0].sum().backward()
+        return lib.calls
+
+    for copy, strides in ((lambda v: v, (128, 160)), (lambda v: v.clone(memory_format=torch.contiguous_format), (100, 100)),
+                          (lambda v: v.t().contiguous().t() if v.dim() == 2 else v, (100, 100))):
+        first, second = packed(copy)
+        assert first[2:4] == (128, 160) and second[2:4] == strides
+        assert second[:2] == (6, 100)
+        if strides == (128, 160):
+            assert second[4:] == first[4:]
+    for change in (torch.Tensor.double, lambda v: v[:3], lambda v: v.reshape(-1)):
+        with pytest.raises(RuntimeError, match="saved"):
+            packed(lambda v: change(v) if v.shape == (6, 100) and v.dtype == torch.float32 else v)
+        with pytest.raises(RuntimeError, match="saved"):
+            packed(lambda v: change(v) if v.dtype == torch.uint8 else v)
+    with pytest.raises(RuntimeError, match="saved"):
+        packed(lambda v: v.int() if v.dtype == torch.int64 and v.shape == (6, 2) else v)
+
+
+@gpu
+@pytest.mark.parametrize("rows, width", ((7, 100), (3, 5000), (4099, 700), (2, 70001)))
+@pytest.mark.parametrize("masked", (False, True))
+def test_gradients_under_saved_tensor_hooks(rows, width, masked):
+    """Sliced logits and masks under hooks that copy: the same bits as without hooks."""
+    g = torch.Generator(device="cuda").manual_seed(width)
+    wide = torch.randn(rows, width + 28, generator=g, device="cuda")
+    on = (torch.rand(rows, width + 60, generator=g, device="cuda") < 0.7)[:, 3:3 + width] if masked else None
+    t = torch.randint(0, width, (rows, 2), generator=g, device="cuda")
+    ups = [torch.randn(sh, generator=g, device="cuda") for sh in ((rows, 2), (rows,), (rows,), (rows, 5))]
+    grads = []
+    for hooks in (None, (lambda v: v.clone(memory_format=torch.contiguous_format), lambda v: v),
+                  (lambda v: (v.device, v.cpu()), lambda v: v[1].to(v[0]))):
+        leaf = wide.detach().requires_grad_(True)
+        x = leaf[:, 5:5 + width]
+        if hooks:
+            with torch.autograd.graph.saved_tensors_hooks(*hooks):
+                out = target_logprobs(x, t, 0.9, on, 5)
+        else:
+            out = target_logprobs(x, t, 0.9, on, 5)
+        grads.append(torch.autograd.grad([out.logprobs, out.entropy, out.lse, out.top_logprobs], leaf, ups)[0])
+    assert torch.equal(grads[0], grads[1]) and torch.equal(grads[0], grads[2])
