@@ -17,6 +17,7 @@ import math
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _native as N
@@ -149,12 +150,15 @@ def target_logprobs(logits: torch.Tensor, targets: torch.Tensor, tau: float = 1.
     has ``lse`` -inf, entropy 0, every log probability -inf and gradient 0.  A row with NaN or +inf
     among its candidates is NaN throughout, with no alternatives.  Alternatives are ordered by logit,
     ties to the lowest column; candidates at -inf are not listed.  A target outside [-1, V) gets NaN
-    and sets the device error word (``_native.raise_device_errors``).
+    and sets the device error word (``_native.raise_device_errors``).  Logits with a forward-mode tangent
+    are refused: the derivative is reverse-mode, once.
     """
     if logits.dtype not in N.DTYPES:
         raise TypeError(f"target_logprobs: logits must be float32, bfloat16 or float16, got {logits.dtype}")
     if targets.dtype not in (torch.int64, torch.int32):
         raise TypeError(f"target_logprobs: targets must be int64 or int32, got {targets.dtype}")
+    if forward_ad.unpack_dual(logits).tangent is not None:
+        raise NotImplementedError("target_logprobs: no forward-mode derivative")
     if logits.dim() < 1 or logits.shape[-1] < 1 or logits.shape[-1] > 1 << 30:
         raise ValueError(f"target_logprobs: logits must be [..., V] with 1 <= V <= 2^30, got {tuple(logits.shape)}")
     lead = tuple(logits.shape[:-1])

@@ -579,3 +579,31 @@ def test_gradients_under_saved_tensor_hooks(rows, width, masked):
             out = target_logprobs(x, t, 0.9, on, 5)
         grads.append(torch.autograd.grad([out.logprobs, out.entropy, out.lse, out.top_logprobs], leaf, ups)[0])
     assert torch.equal(grads[0], grads[1]) and torch.equal(grads[0], grads[2])
+
+
+def test_forward_mode_tangents_are_refused():
+    """There is no forward-mode derivative: a tangent is not dropped in silence."""
+    import torch.autograd.forward_ad as forward_ad
+
+    from minikg_dev_b200.decode import tail_logprobs
+    x, t = torch.rand(3, 8) + 0.5, torch.zeros(3, dtype=torch.int64)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: target_logprobs(dual, t), lambda: tail_logprobs(dual, t)):
+            with pytest.raises(NotImplementedError, match="forward"):
+                call()
+            with torch.no_grad(), pytest.raises(NotImplementedError, match="forward"):
+                call()
+
+
+@gpu
+def test_forward_mode_around_other_tensors():
+    """Inside a dual level, logits without a tangent are read as ever."""
+    import torch.autograd.forward_ad as forward_ad
+    x, t = torch.randn(3, 8, device="cuda"), torch.zeros(3, dtype=torch.int64, device="cuda")
+    want = target_logprobs(x, t)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        assert torch.equal(target_logprobs(x, t).logprobs, want.logprobs)
+        with pytest.raises(NotImplementedError, match="forward"):
+            target_logprobs(dual, t)
