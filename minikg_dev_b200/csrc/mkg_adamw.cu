@@ -40,6 +40,8 @@ constexpr int kChunk = kThreads / kWarp * kBlock;
 // 96 with 4 (spills) and 108 with 2.
 constexpr int kBlocks8 = 3, kBlocks32 = 5;
 constexpr unsigned kFull = 0xffffffffu;
+// Second moments below this, the largest held value less 1 in 14,000, do not saturate; larger ones are taken in fp64.
+constexpr float kSecondClear = 0x1.bff8p120f;
 constexpr int kFirstLow = -120, kFirstHigh = 119, kSecondLow = -90, kSecondHigh = 120;  // of the blocks' scales
 
 // Tensors of one launch.  A launch's parameters may take 32,764 bytes.
@@ -266,7 +268,7 @@ __device__ __forceinline__ void step_held(const Hyper& h, const Held& at, float 
   top2 = warp_max(top2);
   most_off = warp_max(most_off);
   int fe = first_exponent(top1 + most_off), se = second_exponent(top2 * (1.0f + 0x1p-20f));
-  const bool clear = top1 <= FLT_MAX && top2 <= FLT_MAX && first_exponent(fmaxf(top1 - most_off, 0.0f)) == fe &&
+  const bool clear = top1 <= FLT_MAX && top2 <= kSecondClear && first_exponent(fmaxf(top1 - most_off, 0.0f)) == fe &&
                      second_exponent(top2 * (1.0f - 0x1p-20f)) == se;
   uint32_t again1 = 0, again2 = 0;  // values to be taken in fp64: bit 7 - u of byte i
   uint32_t fw[kQuads], sw[kQuads];

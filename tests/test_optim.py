@@ -661,3 +661,30 @@ def test_sixteen_bit_parameters_take_gradients_in_32_bits(dtype):
     chosen.grad_dtype = torch.float32
     AdamW([chosen, wide])
     assert chosen.grad_dtype is torch.float32 and wide.grad_dtype is torch.float32
+
+
+@gpu
+def test_large_second_moments_in_8_bits():
+    """Squares past the largest held value (1.75 * 2^120, about 2.3e36) are held as that, and later steps stay
+    finite: the sums are below fp32's largest value for all of these gradients."""
+    big = (4.7e19, 4.8e19, 4.823e19, 4.83e19, 5e19, 5.2e19, 1e20, 3e20, 5e20)
+    g = torch.full((len(big), BLOCK), 1e10, device="cuda")
+    g[:, 0] = torch.tensor(big)
+    g[:, 1] = -g[:, 0]
+    g[:, 2] = 0.0
+    g[:, 3] = 1.0
+    p = torch.nn.Parameter(torch.zeros_like(g))
+    p.grad = g
+    opt = AdamW([p], lr=0.1, state_bits=8)
+    table, most = second_table(), 1.75 * 2.0 ** 120
+    for _ in range(3):
+        v0 = opt.moments()[1].double().cpu()
+        opt.step()
+        v = opt.moments()[1].double().cpu()
+        want = 0.999 * v0 + (1 - 0.999) * g.reshape(-1).double().cpu().square()
+        _, _, s = hold(want.clamp_max(most), table, -90)
+        s = s.repeat_interleave(BLOCK)
+        least = torch.where(want > 0, table[1], 0.0)
+        want = torch.maximum(table[nearest(table, (want / s).clamp_max(1.75))], least) * s
+        assert torch.equal(v, want)
+        assert torch.isfinite(p).all()
