@@ -688,3 +688,27 @@ def test_large_second_moments_in_8_bits():
         want = torch.maximum(table[nearest(table, (want / s).clamp_max(1.75))], least) * s
         assert torch.equal(v, want)
         assert torch.isfinite(p).all()
+
+
+@gpu
+@pytest.mark.parametrize("bits", (32, 8))
+@pytest.mark.parametrize("eps", (0.0, 2.0 ** -62, 2.0 ** -60, 1e-18, 1e-17, 1e-16, 1e-13, 1e-11, 1e-9, 1e-8))
+@pytest.mark.parametrize("beta2", (0.5, 0.999, 0.999999))
+def test_small_eps(eps, bits, beta2):
+    """Second moments around fp32's smallest normal number beside an eps of their root's size.  What a
+    subnormal v is rounded by (its sum and two products: 3 * 2^-149) counts with half its share of v."""
+    n = 4 * BLOCK
+    g = torch.logspace(-19, -14, n, device="cuda")
+    g[1::2] *= -1
+    p = torch.nn.Parameter(torch.zeros(n, device="cuda"))
+    p.grad = g
+    opt = AdamW([p], lr=1e-3, betas=(0.9, beta2), eps=eps, weight_decay=0.0, state_bits=bits)
+    for t in (1, 2):
+        before, (m0, v0) = p.detach().clone(), (x.clone() for x in opt.moments())
+        opt.step()
+        want, m, v, (size, rate) = definition(before, g, m0, v0, t, betas=(0.9, beta2), eps=eps, wd=0.0)
+        lost = 3 * 2.0 ** -149 / v
+        seen = v > 64 * 2.0 ** -149  # below that the root itself is lost
+        tol = rate * (3 * U * size + (8 * U + 3 * U + lost) * (m.abs() + size)) + 4 * U * (want.abs() + before.double().cpu().abs())
+        close(p.detach().cpu()[seen], want[seen], tol[seen], f"step {t}")
+        assert int(seen.sum()) > n // 2
