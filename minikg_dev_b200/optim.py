@@ -171,6 +171,8 @@ class AdamW(torch.optim.Optimizer):
 
     def __setstate__(self, state) -> None:
         super().__setstate__(state)
+        if self._buffers:
+            self._views()  # unpickled tensors share no memory
         for group in self.param_groups:
             self._open_gradients(group["params"])
 

@@ -712,3 +712,34 @@ def test_small_eps(eps, bits, beta2):
         tol = rate * (3 * U * size + (8 * U + 3 * U + lost) * (m.abs() + size)) + 4 * U * (want.abs() + before.double().cpu().abs())
         close(p.detach().cpu()[seen], want[seen], tol[seen], f"step {t}")
         assert int(seen.sum()) > n // 2
+
+
+@gpu
+@pytest.mark.parametrize("bits", (32, 8))
+def test_an_unpickled_optimizer_checkpoints_its_own_moments(bits):
+    """After a step of the unpickled one, its state and state dict are the original's."""
+    import pickle
+    pairs = make((700, (3, 5), 1000), torch.float32, torch.float32, seed=12)
+    opt = AdamW([p for p, _ in pairs], lr=0.02, state_bits=bits)
+    opt.step()
+    for again in (pickle.loads(pickle.dumps(opt)), copy.deepcopy(opt)):
+        twins = again.param_groups[0]["params"]
+        for q, (p, g) in zip(twins, pairs):
+            q.grad = g.clone()
+        again.step()
+        moved = copy.deepcopy(opt)
+        for q, (_, g) in zip(moved.param_groups[0]["params"], pairs):
+            q.grad = g.clone()
+        moved.step()
+        want = moved.state_dict()["state"]
+        for key, entry in again.state_dict()["state"].items():
+            assert float(entry["step"]) == 2.0
+            for name, x in entry.items():
+                assert torch.equal(x, want[key][name]), name
+        at = 0
+        for q in twins:
+            assert int(again.state[q]["step"]) == 2
+            name = "exp_avg" if bits == 32 else "exp_avg_codes"
+            flat = again._buffers["exp_avg"][at:at + q.numel()]
+            assert torch.equal(again.state[q][name].reshape(-1), flat) and bool(flat.any())
+            at += -(-q.numel() // BLOCK) * BLOCK
