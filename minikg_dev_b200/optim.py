@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+from collections import Counter
 from itertools import accumulate
 
 import torch
@@ -194,14 +195,11 @@ class AdamW(torch.optim.Optimizer):
 
     def load_kernels(self) -> None:
         """Loads what ``step`` launches with the present gradients, without a step: before a capture."""
-        for group, plan in zip(self.param_groups, self._plan):
-            seen = set()
-            for p in group["params"]:
-                if p.grad is None or (p.dtype, p.grad.dtype) in seen:
-                    continue
-                seen.add((p.dtype, p.grad.dtype))
-                none = (ctypes.c_int64 * 1)()
-                self._call(group, p.dtype, p.grad.dtype, none, none, none, none, none)
+        for group in self.param_groups:
+            kinds = Counter((p.dtype, p.grad.dtype) for p in group["params"] if p.grad is not None)
+            for (p_dtype, g_dtype), n in kinds.items():  # the kernel goes by how many tensors there are
+                none = (ctypes.c_int64 * n)()
+                self._call(group, p_dtype, g_dtype, none, none, none, none, none)
 
     def _call(self, group, p_dtype, g_dtype, p_at, g_at, numel, offset, index) -> None:
         self._check_group(group)

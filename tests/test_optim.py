@@ -743,3 +743,58 @@ def test_an_unpickled_optimizer_checkpoints_its_own_moments(bits):
             flat = again._buffers["exp_avg"][at:at + q.numel()]
             assert torch.equal(again.state[q][name].reshape(-1), flat) and bool(flat.any())
             at += -(-q.numel() // BLOCK) * BLOCK
+
+
+@gpu
+def test_load_kernels_of_many_tensors(monkeypatch):
+    """What is loaded is what a step of so many tensors launches, for each pair of types."""
+    few, many = make((5,) * 40, torch.bfloat16, torch.bfloat16, seed=1), make((5,) * 131, torch.float32, torch.float32, seed=2)
+    opt = AdamW([p for p, _ in few + many])
+    asked = []
+    call = opt._call
+
+    def record(group, p_dtype, g_dtype, p_at, *rest):
+        asked.append((p_dtype, g_dtype, len(p_at)))
+        call(group, p_dtype, g_dtype, p_at, *rest)
+    monkeypatch.setattr(opt, "_call", record)
+    opt.load_kernels()
+    loaded, asked[:] = sorted(asked, key=str), []
+    assert all(int(opt.state[p]["step"]) == 0 for p, _ in few + many)
+    opt.step()
+    assert loaded == sorted(asked, key=str) and len(loaded) == 2
+
+
+FIRST_CAPTURE = """
+import sys
+import torch
+from minikg_dev_b200.optim import AdamW
+bits = int(sys.argv[1])
+params = [torch.nn.Parameter(torch.full((3 + i,), 1.0, device="cuda")) for i in range(131)]
+twins = [torch.nn.Parameter(p.detach().clone()) for p in params]
+for p in params + twins:
+    p.grad = torch.linspace(-1, 1, p.numel(), device="cuda")
+a, b = AdamW(params, state_bits=bits), AdamW(twins, state_bits=bits)
+a.load_kernels()
+graph = torch.cuda.CUDAGraph()
+torch.cuda.synchronize()
+with torch.cuda.graph(graph):
+    a.step()
+for _ in range(2):
+    graph.replay()
+    b.step()
+torch.cuda.synchronize()
+assert all(torch.equal(p, q) and int(a.state[p]["step"]) == 2 for p, q in zip(params, twins))
+print("same")
+"""
+
+
+@gpu
+@pytest.mark.parametrize("bits", (32, 8))
+def test_the_first_step_of_many_tensors_is_captured(bits):
+    """In a process of its own, in which nothing has loaded the kernel before."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    out = subprocess.run([sys.executable, "-c", FIRST_CAPTURE, str(bits)], capture_output=True, text=True, timeout=300,
+                         cwd=Path(__file__).resolve().parent.parent)
+    assert out.returncode == 0 and out.stdout.strip().endswith("same"), out.stderr[-2000:]
