@@ -13,6 +13,7 @@ binades; a second moment above 0 is never held as 0.  Sums are taken in fp64 and
 """
 from __future__ import annotations
 
+import copy
 import ctypes
 import math
 from collections import Counter
@@ -282,21 +283,26 @@ class AdamW(torch.optim.Optimizer):
     def load_state_dict(self, state_dict) -> None:
         """Loads a state dict of this class or of ``torch.optim.AdamW`` into the buffers in place: moments
         given as fp32 values are rounded to what 8 bits hold, moments given in 8 bits are read as the
-        values they stand for.  Parameters without an entry start anew."""
+        values they stand for.  Parameters without an entry start anew.  Groups take over every key of
+        the saved ones, as copies; a tensor ``lr`` is written in place."""
         groups = state_dict["param_groups"]
         if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
             raise ValueError("AdamW: the state dict has other parameter groups")
+        dev = self._buffers["steps"].device if self._buffers else None
+        rates = []  # the saved groups, copied: keys of others (a scheduler's initial_lr) come along
         for have, new in zip(self.param_groups, groups):
-            merged = {k: new[k] if k in new else v for k, v in have.items() if k != "params"}
+            new = {k: v.detach().to(device=dev, copy=True) if isinstance(v, torch.Tensor) else copy.deepcopy(v)
+                   for k, v in new.items() if k != "params"}
+            if "betas" in new:
+                new["betas"] = tuple(new["betas"])
+            rates.append(new)
+            merged = have | new
             if isinstance(have["lr"], torch.Tensor):
                 merged["lr"] = have["lr"]  # a captured step reads this tensor
-            merged["betas"] = tuple(merged["betas"])
             self._check_group(merged)
             if new.get("amsgrad") or new.get("maximize") or (new.get("decoupled_weight_decay") is False
                                                              and merged["weight_decay"]):
                 raise ValueError("AdamW: the state dict is of an optimizer with amsgrad, maximize or coupled decay")
-        if not self._buffers:
-            return
         entries = []
         for group, new, plan in zip(self.param_groups, groups, self._plan):
             for p, key, n, at, i in zip(group["params"], new["params"], plan.numel, plan.offset, plan.index):
@@ -309,6 +315,17 @@ class AdamW(torch.optim.Optimizer):
                 if any(e[k].numel() != n for k in names):
                     raise ValueError("AdamW: a state dict entry of another size")
                 entries.append((e, n, at, i))
+        if self._buffers:
+            self._load_moments(entries)
+        for have, new in zip(self.param_groups, rates):
+            for k, v in new.items():
+                if k == "lr" and isinstance(have["lr"], torch.Tensor):
+                    have["lr"].copy_(torch.as_tensor(v).reshape(have["lr"].shape))
+                elif k != "params":
+                    have[k] = v
+
+    def _load_moments(self, entries) -> None:
+        """The flat buffers from (entry, size, offset, step-count index) of each parameter that has one."""
         dev = self._buffers["steps"].device
         m, v = (torch.zeros(max(self._total, 1), dtype=torch.float32, device=dev) for _ in range(2))
         codes = {k: torch.zeros(max(self._total, 1), dtype=torch.uint8, device=dev) for k in ("exp_avg", "exp_avg_sq")}
@@ -341,11 +358,3 @@ class AdamW(torch.optim.Optimizer):
             with N.on_device(dev):
                 N.check(N.load().mkg_adamw_pack(self._state_struct(), m.data_ptr(), v.data_ptr(),
                                                 N.stream_handle(dev)), "adamw_pack")
-        for have, new in zip(self.param_groups, groups):
-            for k in have:
-                if k == "params" or k not in new:
-                    continue
-                if k == "lr" and isinstance(have["lr"], torch.Tensor):
-                    have["lr"].copy_(torch.as_tensor(new["lr"]).reshape(have["lr"].shape))
-                else:
-                    have[k] = tuple(new[k]) if k == "betas" else new[k]

@@ -798,3 +798,49 @@ def test_the_first_step_of_many_tensors_is_captured(bits):
     out = subprocess.run([sys.executable, "-c", FIRST_CAPTURE, str(bits)], capture_output=True, text=True, timeout=300,
                          cwd=Path(__file__).resolve().parent.parent)
     assert out.returncode == 0 and out.stdout.strip().endswith("same"), out.stderr[-2000:]
+
+
+@gpu
+def test_a_loaded_group_keeps_what_the_saved_one_had():
+    """A scheduler resumes from a loaded optimizer, and other keys of a group come along, as copies."""
+    (p, _), = make((40,), torch.float32, torch.float32)
+    src = AdamW([{"params": [p], "note": ["facts"]}], lr=0.1)
+    sched = torch.optim.lr_scheduler.ExponentialLR(src, 0.5)
+    for _ in range(2):
+        src.step()
+        sched.step()
+    saved = src.state_dict()
+    q = torch.nn.Parameter(p.detach().clone())
+    dst = AdamW([q], lr=0.7)
+    dst.load_state_dict(saved)
+    group = dst.param_groups[0]
+    assert group["initial_lr"] == 0.1 and group["lr"] == 0.025 and group["note"] == ["facts"]
+    assert group["params"][0] is q
+    src.param_groups[0]["note"].append("changed")
+    assert group["note"] == ["facts"]
+    again = torch.optim.lr_scheduler.ExponentialLR(dst, 0.5, last_epoch=1)
+    q.grad = torch.ones(40, device="cuda")
+    dst.step()
+    again.step()
+    sched.step()
+    assert dst.param_groups[0]["lr"] == src.param_groups[0]["lr"]
+    torch_side = torch.optim.AdamW([torch.nn.Parameter(p.detach().clone())], lr=0.3)
+    torch_side.load_state_dict(dst.state_dict())
+    assert torch_side.param_groups[0]["initial_lr"] == 0.1
+
+
+@gpu
+@pytest.mark.parametrize("where", ("cuda", "cpu"))
+def test_a_loaded_rate_is_a_copy(where):
+    """Two optimizers do not share a rate's tensor after a load; one saved on the host comes to the device."""
+    (p, _), (q, _) = make((40, 40), torch.float32, torch.float32)
+    src, dst = AdamW([p], lr=torch.tensor(0.25, device="cuda")), AdamW([q], lr=0.7)
+    saved = src.state_dict()
+    saved["param_groups"][0]["lr"] = saved["param_groups"][0]["lr"].to(where)
+    dst.load_state_dict(saved)
+    src.param_groups[0]["lr"].fill_(0.5)
+    assert float(dst.param_groups[0]["lr"]) == 0.25 and dst.param_groups[0]["lr"].is_cuda
+    kept = dst.param_groups[0]["lr"]
+    dst.step()
+    dst.load_state_dict(src.state_dict())
+    assert dst.param_groups[0]["lr"] is kept and float(kept) == 0.5  # in place: captured steps read it
