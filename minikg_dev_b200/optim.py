@@ -16,10 +16,11 @@ from __future__ import annotations
 import copy
 import ctypes
 import math
-from collections import Counter
+from collections import Counter, OrderedDict
 from itertools import accumulate
 
 import torch
+from torch.utils.hooks import RemovableHandle
 
 from . import _native as N
 
@@ -74,6 +75,7 @@ class AdamW(torch.optim.Optimizer):
         self._plan = []     # a _Plan per group
         self._buffers = {}  # flat moments, scales, step counts, the ticket word
         self._total = self._tensors = 0
+        self._before_load, self._after_load = OrderedDict(), OrderedDict()
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
 
     # ------------------------------------------------------------------ parameters and their state
@@ -280,11 +282,31 @@ class AdamW(torch.optim.Optimizer):
         out["state"] = {k: {**e, "step": torch.tensor(float(steps[k]))} for k, e in out["state"].items()}
         return out
 
+    @staticmethod
+    def _hooked(hooks, hook, prepend):
+        handle = RemovableHandle(hooks)
+        hooks[handle.id] = hook
+        if prepend:
+            hooks.move_to_end(handle.id, last=False)
+        return handle
+
+    def register_load_state_dict_pre_hook(self, hook, prepend: bool = False):
+        """``hook(optimizer, state_dict)`` before a load; a dict that it returns is loaded instead."""
+        return self._hooked(self._before_load, hook, prepend)
+
+    def register_load_state_dict_post_hook(self, hook, prepend: bool = False):
+        """``hook(optimizer)`` after a load."""
+        return self._hooked(self._after_load, hook, prepend)
+
     def load_state_dict(self, state_dict) -> None:
         """Loads a state dict of this class or of ``torch.optim.AdamW`` into the buffers in place: moments
         given as fp32 values are rounded to what 8 bits hold, moments given in 8 bits are read as the
         values they stand for.  Parameters without an entry start anew.  Groups take over every key of
         the saved ones, as copies; a tensor ``lr`` is written in place."""
+        state_dict = dict(state_dict)  # hooks may replace its entries
+        for hook in list(self._before_load.values()):
+            given = hook(self, state_dict)
+            state_dict = state_dict if given is None else given
         groups = state_dict["param_groups"]
         if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
             raise ValueError("AdamW: the state dict has other parameter groups")
@@ -323,6 +345,8 @@ class AdamW(torch.optim.Optimizer):
                     have["lr"].copy_(torch.as_tensor(v).reshape(have["lr"].shape))
                 elif k != "params":
                     have[k] = v
+        for hook in list(self._after_load.values()):
+            hook(self)
 
     def _load_moments(self, entries) -> None:
         """The flat buffers from (entry, size, offset, step-count index) of each parameter that has one."""

@@ -844,3 +844,29 @@ def test_a_loaded_rate_is_a_copy(where):
     dst.step()
     dst.load_state_dict(src.state_dict())
     assert dst.param_groups[0]["lr"] is kept and float(kept) == 0.5  # in place: captured steps read it
+
+
+@gpu
+def test_hooks_around_loading():
+    """Hooks before a load see the dict and may give another; hooks after it see the loaded optimizer."""
+    (p, _), (q, _) = make((40, 40), torch.float32, torch.float32)
+    src, dst = AdamW([p], lr=0.25), AdamW([q], lr=0.7)
+    src.step()
+    saved, seen = src.state_dict(), []
+
+    def halve(opt, d):
+        seen.append(("pre", opt is dst, d["param_groups"][0]["lr"]))
+        return {**d, "param_groups": [{**d["param_groups"][0], "lr": d["param_groups"][0]["lr"] / 2}]}
+
+    handles = [dst.register_load_state_dict_pre_hook(halve),
+               dst.register_load_state_dict_pre_hook(lambda opt, d: seen.append("first"), prepend=True),
+               dst.register_load_state_dict_post_hook(
+                   lambda opt: seen.append(("post", opt.param_groups[0]["lr"], int(opt.state[q]["step"])))),
+               dst.register_load_state_dict_post_hook(lambda opt: seen.append("soonest"), prepend=True)]
+    dst.load_state_dict(saved)
+    assert seen == ["first", ("pre", True, 0.25), "soonest", ("post", 0.125, 1)]
+    assert saved["param_groups"][0]["lr"] == 0.25
+    for h in handles:
+        h.remove()
+    dst.load_state_dict(saved)
+    assert len(seen) == 4 and dst.param_groups[0]["lr"] == 0.25
