@@ -16,7 +16,7 @@ from __future__ import annotations
 import copy
 import ctypes
 import math
-from collections import Counter, OrderedDict
+from collections import Counter, OrderedDict, defaultdict
 from itertools import accumulate
 
 import torch
@@ -170,10 +170,12 @@ class AdamW(torch.optim.Optimizer):
                             N.ptr(b.get("exp_avg_sq_scale")), b["steps"].data_ptr(), b["ticket"].data_ptr(),
                             self._total, self._tensors)
 
-    def __getstate__(self):
-        return self.__dict__.copy()
+    def __getstate__(self):  # what others attach (hooks, a scheduler's step) stays here, as with torch's optimizers
+        return {k: self.__dict__[k] for k in ("defaults", "param_groups", "state_bits", "_plan", "_buffers", "_total",
+                                              "_tensors")}
 
     def __setstate__(self, state) -> None:
+        self.state, self._before_load, self._after_load = defaultdict(dict), OrderedDict(), OrderedDict()
         super().__setstate__(state)
         if self._buffers:
             self._views()  # unpickled tensors share no memory

@@ -870,3 +870,28 @@ def test_hooks_around_loading():
         h.remove()
     dst.load_state_dict(saved)
     assert len(seen) == 4 and dst.param_groups[0]["lr"] == 0.25
+
+
+@gpu
+def test_pickling_beside_schedulers_and_hooks():
+    """What others attach to an optimizer (a scheduler wraps its step, hooks may be local functions) stays
+    with it: copies and pickles carry groups and moments, as those of torch's optimizers do."""
+    import pickle
+    pairs = make((300, 40), torch.float32, torch.float32, seed=4)
+    opt = AdamW([p for p, _ in pairs], lr=0.1)
+    sched = torch.optim.lr_scheduler.ExponentialLR(opt, 0.5)
+    calls = []
+    opt.register_step_post_hook(lambda *a: calls.append(1))
+    opt.register_load_state_dict_post_hook(lambda *a: calls.append(2))
+    opt.step()
+    sched.step()
+    assert calls == [1]
+    for again in (pickle.loads(pickle.dumps(opt)), copy.deepcopy(opt)):
+        assert again.param_groups[0]["lr"] == 0.05
+        for q, (_, g) in zip(again.param_groups[0]["params"], pairs):
+            q.grad = g.clone()
+        again.step()
+        again.register_step_post_hook(lambda *a: calls.append(3))
+        again.load_state_dict(again.state_dict())
+        assert [int(again.state[q]["step"]) for q in again.param_groups[0]["params"]] == [2, 2]
+    assert calls == [1] and int(opt.state[pairs[0][0]]["step"]) == 1
