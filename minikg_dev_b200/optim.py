@@ -75,6 +75,7 @@ class AdamW(torch.optim.Optimizer):
         self._plan = []     # a _Plan per group
         self._buffers = {}  # flat moments, scales, step counts, the ticket word
         self._total = self._tensors = 0
+        self._captured = []  # what captured steps read and write, kept as long as the optimizer
         self._before_load, self._after_load = OrderedDict(), OrderedDict()
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
 
@@ -127,7 +128,8 @@ class AdamW(torch.optim.Optimizer):
                 p.grad_dtype = None
 
     def _extend(self, params) -> None:
-        """Room in the flat buffers for one more group; a graph captured before has to be captured again."""
+        """Room in the flat buffers for one more group; a graph captured before has to be captured again (it
+        updates the former moments, which stay allocated)."""
         numel = [p.numel() for p in params]
         room = [-(-n // N.ADAMW_BLOCK) * N.ADAMW_BLOCK for n in numel]
         offset = [self._total + x for x in accumulate(room, initial=0)][:-1]
@@ -175,6 +177,7 @@ class AdamW(torch.optim.Optimizer):
                                               "_tensors")}
 
     def __setstate__(self, state) -> None:
+        self._captured = []
         self.state, self._before_load, self._after_load = defaultdict(dict), OrderedDict(), OrderedDict()
         super().__setstate__(state)
         if self._buffers:
@@ -219,6 +222,8 @@ class AdamW(torch.optim.Optimizer):
         with N.on_device(dev):
             N.check(N.load().mkg_adamw_step(hyper, self._state_struct(), len(numel), p_at, g_at, numel, offset, index,
                                             N.stream_handle(dev)), "adamw_step")
+            if torch.cuda.is_current_stream_capturing():
+                self._captured.append((self._buffers, lr, [p.grad for p in group["params"]]))
 
     def _launch(self, group, params, plan) -> None:
         dev, n = self._buffers["steps"].device, len(params)

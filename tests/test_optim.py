@@ -895,3 +895,36 @@ def test_pickling_beside_schedulers_and_hooks():
         again.load_state_dict(again.state_dict())
         assert [int(again.state[q]["step"]) for q in again.param_groups[0]["params"]] == [2, 2]
     assert calls == [1] and int(opt.state[pairs[0][0]]["step"]) == 1
+
+
+@gpu
+@pytest.mark.parametrize("bits", (32, 8))
+def test_a_captured_step_keeps_its_moments(bits):
+    """A group that is added after a capture moves the moments; what the graph would write to is not
+    handed to others (the graph itself has to be captured again, and is not replayed here)."""
+    pairs = make((5000, 300), torch.float32, torch.float32, seed=6)
+    (p, _), (q, _) = pairs
+    opt = AdamW([p], state_bits=bits)
+    opt.load_kernels()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        opt.step()
+    old = [(b.data_ptr(), b.numel(), b.dtype) for b in opt._buffers.values()]
+    opt.add_param_group({"params": [q]})
+    now = {b.data_ptr() for b in opt._buffers.values()}
+    others = [torch.empty(n, dtype=t, device="cuda") for _, n, t in old for _ in range(20)]
+    taken = {x.data_ptr() for x in others} | now
+    assert not any(at in taken for at, _, _ in old)
+
+
+@gpu
+def test_optimizers_that_were_never_captured_keep_one_set_of_moments():
+    pairs = make((5000, 300), torch.float32, torch.float32, seed=6)
+    opt = AdamW([pairs[0][0]])
+    opt.step()
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    for _ in range(8):
+        opt.add_param_group({"params": [torch.nn.Parameter(torch.zeros(256, device="cuda"))]})
+    assert torch.cuda.memory_allocated() - before < 4 * 2 * 5000 * 4

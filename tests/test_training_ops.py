@@ -283,3 +283,25 @@ def test_training_run(bits):
     for (name, p), (_, q) in zip(model.named_parameters(), twin.named_parameters()):
         assert float((p.double().cpu() - q).abs().max()) <= tol, name
     assert {int(opt.state[p]["step"]) for p in model.parameters()} == {steps}
+
+
+@gpu
+def test_a_captured_update_keeps_what_it_reads():
+    """A rate's tensor that is taken out of the optimizer after the capture, and moments that a new group
+    moves, are not handed to others while the graph is there.  Nothing is replayed."""
+    from minikg_dev_b200.proof import ProofRunner
+    kg, g = small_graph()
+    B, L, K, E, n = 2, 1, 1, kg.num_entities, 2 * kg.num_relations + 1
+    w = torch.nn.Parameter(torch.rand(K, B, L, n, device="cuda"))
+    w.grad = torch.zeros_like(w)
+    opt = AdamW([w], lr=torch.full((1,), 0.01, device="cuda"))
+    graph = ProofRunner(g, B, L, K).capture(
+        torch.zeros(B, dtype=torch.int64, device="cuda"), w, torch.zeros(B, E, device="cuda"),
+        torch.zeros(K, dtype=torch.int64, device="cuda"), torch.zeros(B, E, device="cuda"),
+        torch.rand(kg.num_triples, device="cuda"), w.grad, optimizer=opt)
+    old = [(b.data_ptr(), b.numel(), b.dtype) for b in (*opt._buffers.values(), opt.param_groups[0]["lr"])]
+    opt.param_groups[0]["lr"] = 0.5
+    opt.add_param_group({"params": [torch.nn.Parameter(torch.zeros(300, device="cuda"))]})
+    others = [torch.empty(k, dtype=t, device="cuda") for _, k, t in old for _ in range(200)]
+    assert not {x.data_ptr() for x in others} & {at for at, _, _ in old}
+    del graph
