@@ -49,10 +49,6 @@ def _row_stride(t: torch.Tensor) -> int | None:
     return step
 
 
-def _strides(size) -> tuple[int, ...]:
-    return tuple(math.prod(size[i + 1:]) for i in range(len(size)))
-
-
 def _as_rows(t: torch.Tensor | None):
     """(t, row stride) of a tensor the library can read, copied only where it cannot be read as it is."""
     if t is None:
@@ -78,17 +74,9 @@ def _forward(logits, targets, mask, tau: float, topk: int, stats):
     None) receives what the backward needs."""
     lib, dev, lead = N.load(), logits.device, logits.shape[:-1]
     p, x, m = _reading(logits, targets, mask, tau, topk)
-    rows = p.rows
-    if stats is None:  # nobody differentiates: one allocation, the outputs are its parts
-        s, k = targets.numel(), rows * topk
-        buffer = torch.empty(s + 2 * rows + k, dtype=torch.float32, device=dev)
-        logprobs, entropy, lse, top_logprobs = (
-            torch.as_strided(buffer, size, _strides(size), at)
-            for size, at in ((targets.shape, 0), (lead, s), (lead, s + rows), ((*lead, topk), s + 2 * rows)))
-    else:
-        logprobs = torch.empty_like(targets, dtype=torch.float32)
-        entropy, lse = (torch.empty(lead, dtype=torch.float32, device=dev) for _ in range(2))
-        top_logprobs = torch.empty((*lead, topk), dtype=torch.float32, device=dev)
+    logprobs = torch.empty_like(targets, dtype=torch.float32)
+    entropy, lse = (torch.empty(lead, dtype=torch.float32, device=dev) for _ in range(2))
+    top_logprobs = torch.empty((*lead, topk), dtype=torch.float32, device=dev)
     top_ids = torch.empty((*lead, topk), dtype=torch.int64, device=dev)
     with N.on_device(dev):
         need = lib.mkg_logprob_workspace_bytes(p)

@@ -607,3 +607,19 @@ def test_forward_mode_around_other_tensors():
         assert torch.equal(target_logprobs(x, t).logprobs, want.logprobs)
         with pytest.raises(NotImplementedError, match="forward"):
             target_logprobs(dual, t)
+
+
+@gpu
+def test_outputs_without_gradients_are_tensors_of_their_own():
+    """Changing one in place leaves a graph that saved another as it is, and none keeps the others' memory."""
+    x, t = torch.randn(5, 300, device="cuda"), torch.zeros(5, 2, dtype=torch.int64, device="cuda")
+    w = torch.ones(5, 2, device="cuda", requires_grad=True)
+    out = target_logprobs(x, t, topk=4)
+    want = out.logprobs.clone()
+    loss = (w * out.logprobs).sum()
+    for o in (out.entropy, out.lse, out.top_logprobs):
+        o.zero_()
+    loss.backward()
+    assert torch.equal(w.grad, want)
+    parts = [out.logprobs, out.entropy, out.lse, out.top_ids, out.top_logprobs]
+    assert len({o.untyped_storage().data_ptr() for o in parts}) == 5 and not any(o._is_view() for o in parts)
