@@ -53,6 +53,7 @@ def _as_rows(t: torch.Tensor | None):
     """(t, row stride) of a tensor the library can read, copied only where it cannot be read as it is."""
     if t is None:
         return None, 0
+    t = t.resolve_neg()  # torch's lazily negated views hold the opposite in memory
     stride = _row_stride(t)
     if stride is None:
         t = t.contiguous()
@@ -115,7 +116,7 @@ class _TargetLogprobs(torch.autograd.Function):
         targets, top_ids, entropy, stats = (t.contiguous() for t in (saved[1], *saved[3:]))
         p, x, m = _reading(logits, targets, mask, *ctx.call)
         dev = logits.device
-        ups = [g if g is None or g.is_contiguous() else g.contiguous() for g in (g_logprobs, g_entropy, g_lse, g_top)]
+        ups = [g if g is None else g.resolve_neg().contiguous() for g in (g_logprobs, g_entropy, g_lse, g_top)]
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
         with N.on_device(dev):
             N.check(N.load().mkg_logprob_backward(p, x.data_ptr(), N.ptr(m), targets.data_ptr(),

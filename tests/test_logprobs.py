@@ -623,3 +623,32 @@ def test_outputs_without_gradients_are_tensors_of_their_own():
     assert torch.equal(w.grad, want)
     parts = [out.logprobs, out.entropy, out.lse, out.top_ids, out.top_logprobs]
     assert len({o.untyped_storage().data_ptr() for o in parts}) == 5 and not any(o._is_view() for o in parts)
+
+
+@gpu
+def test_lazily_negated_logits_and_gradients():
+    """Tensors that torch negates when they are read (imaginary parts of conjugates): single elements count
+    as contiguous and arrive as they are in memory."""
+    z = torch.complex(torch.randn(4, device="cuda"), torch.randn(4, device="cuda"))
+    t = torch.zeros(4, dtype=torch.int64, device="cuda")
+    x = z.conj().imag[:, None]
+    assert x.is_neg()
+    assert torch.equal(target_logprobs(x, t).lse, -z.imag)
+    assert torch.equal(target_logprobs(x[:1], t[:1], topk=1).lse, -z.imag[:1])
+    whole = torch._neg_view(torch.randn(3, 50, device="cuda"))
+    t = torch.ones(3, dtype=torch.int64, device="cuda")
+    want = target_logprobs(whole.resolve_neg(), t, topk=3)
+    for a, b in zip(target_logprobs(whole, t, topk=3), want):
+        assert torch.equal(a, b)
+    leaf = torch.randn(1, 50, device="cuda", requires_grad=True)
+    grads = []
+    for up in (torch._neg_view(torch.full((1,), 0.5, device="cuda")), torch.full((1,), -0.5, device="cuda")):
+        out = target_logprobs(leaf, t[:1], topk=1)
+        grads += [torch.autograd.grad(o, leaf, up.view(o.shape), retain_graph=True)[0]
+                  for o in (out.logprobs, out.entropy, out.lse, out.top_logprobs)]
+    for a, b in zip(grads[:4], grads[4:]):
+        assert torch.equal(a, b) and bool(a.any())
+    neg = whole.detach().requires_grad_(True)
+    pos = whole.detach().resolve_neg().clone().requires_grad_(True)
+    ga, gb = (torch.autograd.grad(target_logprobs(v, t).logprobs.sum(), v)[0] for v in (neg, pos))
+    assert torch.equal(ga, gb)
