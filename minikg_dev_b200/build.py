@@ -73,7 +73,10 @@ def _build_tensors() -> None:
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", f"-I{sysconfig.get_paths()['include']}",
            *(f"-isystem{root / d}" for d in ("include", "include/torch/csrc/api/include")), str(TENSORS),
            "-o", str(TENSORS_LIB), f"-L{root / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10"]
-    res = subprocess.run(cmd, capture_output=True, text=True)
+    try:
+        res = subprocess.run(cmd, capture_output=True, text=True)
+    except OSError as e:
+        raise RuntimeError(f"g++, which {TENSORS.name} is built with, does not run: {e}") from e
     if res.returncode != 0:
         raise RuntimeError(f"g++ failed on {TENSORS.name}:\n{res.stderr}\n{res.stdout}")
 
@@ -85,8 +88,6 @@ def build(force: bool = False, verbose_ptxas: bool = False, quiet: bool = True) 
     hdrs = headers()
     todo = [s for s in srcs if force or verbose_ptxas or _stale(BUILD / (s.stem + ".o"), [s, *hdrs])]
     logs = []
-    if force or _stale(TENSORS_LIB, [TENSORS]):
-        _build_tensors()
     if todo:
         with ThreadPoolExecutor(max_workers=min(8, len(todo))) as ex:
             for obj, log in ex.map(lambda s: _compile(s, verbose_ptxas), todo):
@@ -100,6 +101,8 @@ def build(force: bool = False, verbose_ptxas: bool = False, quiet: bool = True) 
         res = subprocess.run(cmd, capture_output=True, text=True)
         if res.returncode != 0:
             raise RuntimeError(f"link failed:\n{res.stderr}\n{res.stdout}")
+    if force or _stale(TENSORS_LIB, [TENSORS]):  # last: programs without torch need only the library above
+        _build_tensors()
     if not quiet or verbose_ptxas:
         for obj, log in logs:
             if log.strip():

@@ -105,3 +105,26 @@ def test_product_fails_loudly_without_a_gpu():
     with pytest.raises(RuntimeError, match="CUDA tensor"):
         build_csr_structure(torch.zeros(3, dtype=torch.int32), torch.zeros(3, dtype=torch.int32),
                             torch.zeros(3, dtype=torch.int32), 4)
+
+
+def test_the_cuda_library_is_built_without_the_tensor_reader(monkeypatch, tmp_path):
+    """A compiler or headers that are missing for the reader of torch tensors cost that alone, and say so."""
+    from minikg_dev_b200 import build as B
+
+    def fails():
+        raise RuntimeError("no headers")
+    B.build()
+    monkeypatch.setattr(B, "LIB", tmp_path / "lib.so")
+    monkeypatch.setattr(B, "TENSORS_LIB", tmp_path / "tensors.so")
+    monkeypatch.setattr(B, "_build_tensors", fails)
+    with pytest.raises(RuntimeError, match="no headers"):
+        B.build()
+    assert hasattr(ctypes.CDLL(str(tmp_path / "lib.so")), "mkg_adamw_step")
+
+
+def test_a_missing_compiler_is_named(monkeypatch, tmp_path):
+    from minikg_dev_b200 import build as B
+    monkeypatch.setattr(B, "TENSORS_LIB", tmp_path / "tensors.so")
+    monkeypatch.setenv("PATH", str(tmp_path))
+    with pytest.raises(RuntimeError, match="g\\+\\+"):
+        B._build_tensors()
