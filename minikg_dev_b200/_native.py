@@ -7,6 +7,7 @@ back to another implementation: without the library (or without a GPU) the call 
 from __future__ import annotations
 
 import ctypes as C
+import sys
 import os
 import threading
 from pathlib import Path
@@ -222,15 +223,29 @@ def load(path: Path | str | None = None):
 _gather = None
 
 
+def torch_tag() -> str:
+    """The torch and the interpreter that ``_lib/libminikg_tensors.so`` has to be built for."""
+    return f"torch {torch.__version__}, Python {sys.version_info.major}.{sys.version_info.minor}"
+
+
 def gather_gradients():
     """``mkg_gather_gradients`` of ``_lib/libminikg_tensors.so``, which reads a list of torch tensors
-    under the interpreter's lock; raises if it was not built."""
+    under the interpreter's lock; raises if it was not built, or built for another torch."""
     global _gather
     if _gather is None:
         if not TENSORS_LIB_PATH.exists():
             raise RuntimeError(f"minikg_b200 native library missing at {TENSORS_LIB_PATH}; run "
                                "`python -m minikg_dev_b200.build`")
-        fn = C.PyDLL(str(TENSORS_LIB_PATH)).mkg_gather_gradients
+        try:
+            lib = C.PyDLL(str(TENSORS_LIB_PATH))
+            lib.mkg_tensors_built_for.restype = C.c_char_p
+            built_for = lib.mkg_tensors_built_for().decode()
+        except (OSError, AttributeError) as e:
+            built_for = f"another torch ({e})"
+        if built_for != torch_tag():
+            raise RuntimeError(f"minikg_b200 native library {TENSORS_LIB_PATH} was built for {built_for}, this is "
+                               f"{torch_tag()}; run `python -m minikg_dev_b200.build`")
+        fn = lib.mkg_gather_gradients
         fn.restype, fn.argtypes = i64, [C.py_object, i64, i64, vp, vp, vp, vp, vp]
         _gather = fn
     return _gather

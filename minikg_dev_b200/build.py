@@ -66,19 +66,32 @@ def _compile(src: Path, verbose_ptxas: bool) -> tuple[Path, str]:
     return obj, res.stderr
 
 
+def _tensors_stamp() -> Path:  # what TENSORS_LIB was built for
+    return TENSORS_LIB.with_suffix(".built_for")
+
+
+def _tensors_stale() -> bool:
+    from ._native import torch_tag
+    stamp = _tensors_stamp()
+    return _stale(TENSORS_LIB, [TENSORS]) or not stamp.exists() or stamp.read_text() != torch_tag()
+
+
 def _build_tensors() -> None:
     import torch
+
+    from ._native import torch_tag
     root = Path(torch.__file__).resolve().parent
     cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-shared",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", f"-I{sysconfig.get_paths()['include']}",
            *(f"-isystem{root / d}" for d in ("include", "include/torch/csrc/api/include")), str(TENSORS),
-           "-o", str(TENSORS_LIB), f"-L{root / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10"]
+           f'-DMKG_BUILT_FOR="{torch_tag()}"', "-o", str(TENSORS_LIB), f"-L{root / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10"]
     try:
         res = subprocess.run(cmd, capture_output=True, text=True)
     except OSError as e:
         raise RuntimeError(f"g++, which {TENSORS.name} is built with, does not run: {e}") from e
     if res.returncode != 0:
         raise RuntimeError(f"g++ failed on {TENSORS.name}:\n{res.stderr}\n{res.stdout}")
+    _tensors_stamp().write_text(torch_tag())
 
 
 def build(force: bool = False, verbose_ptxas: bool = False, quiet: bool = True) -> Path:
@@ -101,7 +114,7 @@ def build(force: bool = False, verbose_ptxas: bool = False, quiet: bool = True) 
         res = subprocess.run(cmd, capture_output=True, text=True)
         if res.returncode != 0:
             raise RuntimeError(f"link failed:\n{res.stderr}\n{res.stdout}")
-    if force or _stale(TENSORS_LIB, [TENSORS]):  # last: programs without torch need only the library above
+    if force or _tensors_stale():  # last: programs without torch need only the library above
         _build_tensors()
     if not quiet or verbose_ptxas:
         for obj, log in logs:

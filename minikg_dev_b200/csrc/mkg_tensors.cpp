@@ -37,6 +37,9 @@ bool on(const at::Tensor& t, int64_t device) {
 
 }  // namespace
 
+// The torch and the interpreter that this was built for: another's tensors are laid out in another way.
+extern "C" __attribute__((visibility("default"))) const char* mkg_tensors_built_for() { return MKG_BUILT_FOR; }
+
 // params: a list of n tensors.  For each with a gradient: their addresses and kinds[i] = (type of the
 // parameter) + 4 (type of the gradient) + 16 if the gradient has to be made contiguous first (its address
 // is not given then); -1 without a gradient.  Returns the status, at[0] the index it is of; at[1] tells

@@ -128,3 +128,20 @@ def test_a_missing_compiler_is_named(monkeypatch, tmp_path):
     monkeypatch.setenv("PATH", str(tmp_path))
     with pytest.raises(RuntimeError, match="g\\+\\+"):
         B._build_tensors()
+
+
+def test_the_tensor_reader_belongs_to_one_torch(monkeypatch):
+    """Built for another torch it is built again, and never called."""
+    import torch
+
+    from minikg_dev_b200 import _native
+    from minikg_dev_b200 import build as B
+    B.build()
+    assert not B._tensors_stale()
+    monkeypatch.setattr(_native, "_gather", None)
+    assert _native.gather_gradients() is not None
+    monkeypatch.setattr(torch, "__version__", "1.0.0")
+    assert B._tensors_stale()
+    monkeypatch.setattr(_native, "_gather", None)
+    with pytest.raises(RuntimeError, match="1.0.0.*python -m minikg_dev_b200.build"):
+        _native.gather_gradients()
