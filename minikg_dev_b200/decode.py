@@ -66,8 +66,8 @@ def tail_logprobs(raw: torch.Tensor, tails: torch.Tensor, mask: torch.Tensor | N
         if mask.dtype != torch.bool:
             raise TypeError(f"tail_logprobs: mask must be bool, got {mask.dtype}")
         scored = scored & mask
-    # below the least normal score log would be -inf and its gradient 0 * inf: those are no candidates
-    return target_logprobs(raw.clamp_min(torch.finfo(torch.float32).tiny).log(), tails, 1.0, scored, topk)
+    # scores that are no candidates become the least positive number: log's gradient at 0 would be 0 / 0
+    return target_logprobs(raw.clamp_min(2.0 ** -149).log(), tails, 1.0, scored, topk)
 
 
 def candidate_rows(tails: torch.Tensor, scores: torch.Tensor, counts: torch.Tensor) -> dict:

@@ -305,3 +305,26 @@ def test_a_captured_update_keeps_what_it_reads():
     others = [torch.empty(k, dtype=t, device="cuda") for _, k, t in old for _ in range(200)]
     assert not {x.data_ptr() for x in others} & {at for at, _, _ in old}
     del graph
+
+
+@gpu
+def test_tail_logprobs_of_scores_below_the_least_normal_number():
+    """They are candidates like others, at their own weight.  log of a score down to 2^-149 is at most 104
+    in size: half a step of fp32 there is 2^-18, and its own error twice that; two of them, and the sum's
+    log, make a log probability: 2^-15."""
+    raw = torch.tensor([[1e-40, 3e-40, 0.0, 6e-40], [8e-39, 4e-39, 0.0, 0.0], [2e-38, 8e-39, 0.5, 0.0], [0.0, 1e-44, 0.0, 0.0]],
+                       device="cuda", requires_grad=True)
+    tails = torch.tensor([[0, 1, 3], [0, 1, 2], [0, 1, 2], [0, 1, -1]], device="cuda")
+    out = tail_logprobs(raw, tails, topk=3)
+    x = raw.detach().double().cpu()
+    logp = torch.log(x / x.sum(1, keepdim=True))
+    want = torch.where(tails.cpu() < 0, 0.0, logp.gather(1, tails.cpu().clamp_min(0)))
+    assert torch.equal(out.logprobs.isinf().cpu(), want.isinf())
+    fine = want.isfinite()
+    assert float((out.logprobs.double().cpu() - want)[fine].abs().max()) <= 2.0 ** -15
+    assert out.top_ids[0].tolist() == [3, 1, 0] and out.top_ids[1].tolist() == [0, 1, -1]
+    # d log p_t / d raw_j = (j == t) / raw_j - 1 / sum over the candidates, 0 elsewhere
+    grad, = torch.autograd.grad(out.logprobs[1, 0], raw)
+    want = torch.tensor([1 / x[1, 0] - 1 / x[1].sum(), -1 / x[1].sum(), 0.0, 0.0], dtype=torch.float64)
+    assert not grad[[0, 2, 3]].any()
+    assert float((grad[1].double().cpu() - want).abs().max()) <= 2.0 ** -14 * float(want.abs().max())
