@@ -627,7 +627,7 @@ typedef struct mkg_logprob_params {
  * MKG_DEV_BAD_TARGET), entropy [rows], lse [rows], the topk largest candidates above -inf by
  * logit (ties: the lowest column) as top_ids [rows, topk] / top_logprobs [rows, topk] (-1 / -inf
  * where a row has fewer), and, unless it is NULL, stats [rows, 2] for the backward (the row's largest
- * logit and log2 of the sum of e^{z - its largest}).  A row without a candidate above -inf has lse -inf,
+ * logit and the sum of e^{z - its largest}).  A row without a candidate above -inf has lse -inf,
  * entropy 0 and every log p -inf; a row with NaN or +inf among its candidates has NaN
  * everywhere and no alternatives.  mask may be NULL. */
 size_t mkg_logprob_workspace_bytes(const mkg_logprob_params* p);

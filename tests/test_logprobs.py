@@ -652,3 +652,21 @@ def test_lazily_negated_logits_and_gradients():
     pos = whole.detach().resolve_neg().clone().requires_grad_(True)
     ga, gb = (torch.autograd.grad(target_logprobs(v, t).logprobs.sum(), v)[0] for v in (neg, pos))
     assert torch.equal(ga, gb)
+
+
+@gpu
+@pytest.mark.parametrize("rows, width", ((3, 1789), (4100, 1789), (4100, 97), (5, 14013), (4100, 2851), (2, 3000017), (1, 4594485)))
+def test_equal_columns_share_the_gradient(rows, width):
+    """p is 1 / width for equal logits.  Every power is 1 and the sum a whole number below 2^24, so both are
+    exact; the reciprocal, the upstream gradient's product and p itself are rounded once each: 4 u, with one u
+    in hand for the scale of tau.  A logarithm of the sum in fp32 in between would cost up to 11 u (half
+    a step of log2 s, times ln 2) on every column alike."""
+    x = torch.full((rows, width), 1.5, device="cuda", requires_grad=True)
+    t = torch.zeros((rows, 1), dtype=torch.int64, device="cuda")
+    out = target_logprobs(x, t)
+    grad, = torch.autograd.grad(out.lse, x, torch.ones(rows, device="cuda"))
+    assert float((grad.double() * width - 1).abs().max()) <= 4 * U
+    out = target_logprobs(x, t)
+    grad, = torch.autograd.grad(out.logprobs, x, torch.ones(rows, 1, device="cuda"))
+    assert float((grad[:, 1:].double() * width + 1).abs().max()) <= 4 * U
+    assert float((grad[:, 0].double() - (1 - 1 / width)).abs().max()) <= 4 * U
