@@ -140,7 +140,7 @@ def target_logprobs(logits: torch.Tensor, targets: torch.Tensor, tau: float = 1.
     among its candidates is NaN throughout, with no alternatives.  Alternatives are ordered by logit,
     ties to the lowest column; candidates at -inf are not listed.  A target outside [-1, V) gets NaN
     and sets the device error word (``_native.raise_device_errors``).  Logits with a forward-mode tangent
-    are refused: the derivative is reverse-mode, once.
+    are refused: the derivative is reverse-mode, once, and of the logits alone (``tau`` is a number).
     """
     if logits.dtype not in N.DTYPES:
         raise TypeError(f"target_logprobs: logits must be float32, bfloat16 or float16, got {logits.dtype}")
@@ -158,6 +158,9 @@ def target_logprobs(logits: torch.Tensor, targets: torch.Tensor, tau: float = 1.
         raise ValueError(f"target_logprobs: at most {N.LOGPROB_TARGETS_MAX} targets per row, got {s}")
     if not 0 <= int(topk) <= N.LOGPROB_TOPK_MAX:
         raise ValueError(f"target_logprobs: topk must be in [0, {N.LOGPROB_TOPK_MAX}], got {topk}")
+    if isinstance(tau, torch.Tensor) and ((tau.requires_grad and torch.is_grad_enabled())
+                                          or forward_ad.unpack_dual(tau).tangent is not None):
+        raise NotImplementedError("target_logprobs: tau is a number and has no derivative")
     tau = float(tau)
     if not 2.0 ** -60 <= tau <= 2.0 ** 60:
         raise ValueError(f"target_logprobs: tau must be in [2^-60, 2^60], got {tau}")

@@ -248,7 +248,7 @@ def rule_logprobs(model, target_rel: torch.Tensor, bodies: torch.Tensor, tau: fl
     channel, the product that the hop loop gives each of its paths.  Runs once per distinct relation, on
     the logits of ``build_rule_logits``; gradients flow to every producer parameter through the log
     probabilities and the entropy, in a fixed order."""
-    tau = float(model.tau_1 if tau is None else tau)
+    tau = model.tau_1 if tau is None else tau
     if bodies.dim() != 3 or bodies.shape[0] != target_rel.numel():
         raise ValueError(f"rule_logprobs: bodies must be [{target_rel.numel()}, S, K], got {tuple(bodies.shape)}")
     if bodies.dtype not in (torch.int64, torch.int32):

@@ -670,3 +670,18 @@ def test_equal_columns_share_the_gradient(rows, width):
     grad, = torch.autograd.grad(out.logprobs, x, torch.ones(rows, 1, device="cuda"))
     assert float((grad[:, 1:].double() * width + 1).abs().max()) <= 4 * U
     assert float((grad[:, 0].double() - (1 - 1 / width)).abs().max()) <= 4 * U
+
+
+def test_a_trained_temperature_is_refused():
+    """tau is a number: a tensor that asks for its gradient, or has a tangent, would silently get none."""
+    import torch.autograd.forward_ad as forward_ad
+    x, t = torch.rand(3, 8), torch.zeros(3, dtype=torch.int64)
+    tau = torch.tensor(0.7, requires_grad=True)
+    with pytest.raises(NotImplementedError, match="tau"):
+        target_logprobs(x, t, tau)
+    with forward_ad.dual_level(), pytest.raises(NotImplementedError, match="tau"):
+        target_logprobs(x, t, forward_ad.make_dual(torch.tensor(0.7), torch.tensor(1.0)))
+    with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA tensor"):  # read as a number: the next check's turn
+        target_logprobs(x, t, tau)
+    with pytest.raises(RuntimeError, match="CUDA tensor"):
+        target_logprobs(x, t, tau.detach())

@@ -328,3 +328,16 @@ def test_tail_logprobs_of_scores_below_the_least_normal_number():
     want = torch.tensor([1 / x[1, 0] - 1 / x[1].sum(), -1 / x[1].sum(), 0.0, 0.0], dtype=torch.float64)
     assert not grad[[0, 2, 3]].any()
     assert float((grad[1].double().cpu() - want).abs().max()) <= 2.0 ** -14 * float(want.abs().max())
+
+
+@gpu
+def test_rule_logprobs_of_a_trained_temperature():
+    """tau gets no gradient here: a temperature that asks for one is refused, a frozen one is read."""
+    model = Producer()
+    rel, bodies = torch.tensor([0, 1], device="cuda"), torch.zeros((2, 1, 2), dtype=torch.int64, device="cuda")
+    want = rules.rule_logprobs(model, rel, bodies).logprobs
+    model.tau_1 = torch.nn.Parameter(torch.tensor(0.8))
+    with pytest.raises(NotImplementedError, match="tau"):
+        rules.rule_logprobs(model, rel, bodies)
+    model.tau_1.requires_grad_(False)
+    torch.testing.assert_close(rules.rule_logprobs(model, rel, bodies).logprobs, want, rtol=4 * U, atol=16 * U)
