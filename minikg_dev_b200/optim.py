@@ -286,7 +286,8 @@ class AdamW(torch.optim.Optimizer):
         on the host), which continues from moments in 32 bits."""
         out = super().state_dict()
         steps = self._buffers["steps"].tolist() if self._buffers else []
-        out["state"] = {k: {**e, "step": torch.tensor(float(steps[k]))} for k, e in out["state"].items()}
+        out["state"] = {k: {**e, "step": torch.tensor(float(steps[k]), dtype=torch.float32, device="cpu")}
+                        for k, e in out["state"].items()}
         return out
 
     @staticmethod
@@ -360,7 +361,8 @@ class AdamW(torch.optim.Optimizer):
         dev = self._buffers["steps"].device
         m, v = (torch.zeros(max(self._total, 1), dtype=torch.float32, device=dev) for _ in range(2))
         codes = {k: torch.zeros(max(self._total, 1), dtype=torch.uint8, device=dev) for k in ("exp_avg", "exp_avg_sq")}
-        codes |= {k: torch.zeros(max(self._total // N.ADAMW_BLOCK, 1), device=dev) for k in _CODES[1::2]}
+        codes |= {k: torch.zeros(max(self._total // N.ADAMW_BLOCK, 1), dtype=torch.float32, device=dev)
+                  for k in _CODES[1::2]}
         codes |= {k: self._buffers[k] for k in ("steps", "ticket")}
         coded = [x for x in entries if "exp_avg" not in x[0]]
         for e, n, at, _ in coded:

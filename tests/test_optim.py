@@ -928,3 +928,48 @@ def test_optimizers_that_were_never_captured_keep_one_set_of_moments():
     for _ in range(8):
         opt.add_param_group({"params": [torch.nn.Parameter(torch.zeros(256, device="cuda"))]})
     assert torch.cuda.memory_allocated() - before < 4 * 2 * 5000 * 4
+
+
+@gpu
+@pytest.mark.parametrize("default", (torch.bfloat16, torch.float64))
+@pytest.mark.parametrize("bits", (32, 8))
+def test_state_dicts_under_another_default_type(bits, default):
+    """torch's default type decides nothing: steps are float32 on the host, scales fp32."""
+    (p, g), (q, _) = make((700, 700), torch.float32, torch.float32, seed=8)
+    src = AdamW([p], state_bits=8)
+    src.step()
+    src._buffers["steps"].fill_(1001)  # not a bf16 number
+    want = [x.clone() for x in src.moments()]
+    q.data.copy_(p.detach())
+    q.grad = g.clone()
+    torch.set_default_dtype(default)
+    try:
+        saved = src.state_dict()
+        dst = AdamW([q], state_bits=bits)
+        dst.load_state_dict(saved)
+        entry = saved["state"][0]["step"]
+        got = [x.clone() for x in dst.moments()]
+        dst.step()
+    finally:
+        torch.set_default_dtype(torch.float32)
+    src.step()
+    assert entry.dtype == torch.float32 and float(entry) == 1001.0 and not entry.is_cuda
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert int(dst.state[q]["step"]) == 1002
+    if bits == 8:
+        assert torch.equal(p, q)
+    else:
+        close(q, p.detach().double().cpu(), 64 * U * (1e-3 + p.detach().double().cpu().abs()), "step")
+
+
+def test_every_tensor_names_its_type():
+    """A factory call that leaves its type to torch's default is read as something else by a kernel."""
+    import ast
+    from pathlib import Path
+    for module in ("optim", "logprobs"):
+        tree = ast.parse((Path(__file__).resolve().parent.parent / "minikg_dev_b200" / f"{module}.py").read_text())
+        for call in ast.walk(tree):
+            if isinstance(call, ast.Call) and isinstance(call.func, ast.Attribute) and isinstance(call.func.value, ast.Name) \
+                    and call.func.value.id == "torch" and call.func.attr in ("zeros", "ones", "empty", "full", "tensor"):
+                named = "dtype" in {k.arg for k in call.keywords}
+                assert named or ast.unparse(call) == "torch.empty(0)", f"{module}.py:{call.lineno}: {ast.unparse(call)}"
