@@ -113,10 +113,10 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError("AdamW: parameters share memory")
             if isinstance(group["lr"], torch.Tensor) and every and group["lr"].device != every[0].device:
                 raise ValueError(f"AdamW: a tensor lr must be on {every[0].device}, got {group['lr'].device}")
+            self._extend(group["params"])
         except Exception:
             del self.param_groups[before:]
             raise
-        self._extend(group["params"])
         self._open_gradients(group["params"])
 
     @staticmethod
@@ -133,25 +133,27 @@ class AdamW(torch.optim.Optimizer):
         numel = [p.numel() for p in params]
         room = [-(-n // N.ADAMW_BLOCK) * N.ADAMW_BLOCK for n in numel]
         offset = [self._total + x for x in accumulate(room, initial=0)][:-1]
-        self._plan.append(_Plan(numel, offset, range(self._tensors, self._tensors + len(numel))))
-        self._total += sum(room)
-        self._tensors += len(numel)
+        plan = _Plan(numel, offset, range(self._tensors, self._tensors + len(numel)))
+        total, tensors = self._total + sum(room), self._tensors + len(numel)
+        buffers = self._allocated(params[0].device, total, tensors) if params else self._buffers
+        self._plan.append(plan)  # from here on nothing needs memory
+        self._total, self._tensors, self._buffers = total, tensors, buffers
         if params:
-            self._allocate(params[0].device)
+            self._views()
 
-    def _allocate(self, dev) -> None:
+    def _allocated(self, dev, total: int, tensors: int) -> dict:
+        """Flat buffers of that many moments and tensors, with what the present ones hold."""
         held = torch.float32 if self.state_bits == 32 else torch.uint8
-        want = {"exp_avg": (self._total, held), "exp_avg_sq": (self._total, held),
-                "steps": (self._tensors, torch.int64), "ticket": (1, torch.int32)}
+        want = {"exp_avg": (total, held), "exp_avg_sq": (total, held), "steps": (tensors, torch.int64),
+                "ticket": (1, torch.int32)}
         if self.state_bits == 8:
-            want |= {k: (self._total // N.ADAMW_BLOCK, torch.float32) for k in ("exp_avg_scale", "exp_avg_sq_scale")}
-        old, self._buffers = self._buffers, {}
+            want |= {k: (total // N.ADAMW_BLOCK, torch.float32) for k in ("exp_avg_scale", "exp_avg_sq_scale")}
+        buffers = {}
         for name, (n, dtype) in want.items():
-            b = torch.zeros(max(n, 1), dtype=dtype, device=dev)
-            if name in old and name != "ticket":
-                b[:old[name].numel()].copy_(old[name])
-            self._buffers[name] = b
-        self._views()
+            b = buffers[name] = torch.zeros(max(n, 1), dtype=dtype, device=dev)
+            if name in self._buffers and name != "ticket":
+                b[:self._buffers[name].numel()].copy_(self._buffers[name])
+        return buffers
 
     def _views(self) -> None:
         """``state[p]``: each parameter's part of the flat buffers."""

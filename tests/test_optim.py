@@ -973,3 +973,30 @@ def test_every_tensor_names_its_type():
                     and call.func.value.id == "torch" and call.func.attr in ("zeros", "ones", "empty", "full", "tensor"):
                 named = "dtype" in {k.arg for k in call.keywords}
                 assert named or ast.unparse(call) == "torch.empty(0)", f"{module}.py:{call.lineno}: {ast.unparse(call)}"
+
+
+@gpu
+@pytest.mark.parametrize("call", (0, 1, 3))
+def test_a_group_without_memory_leaves_the_optimizer_as_it_was(call, monkeypatch):
+    (p, _), (q, _) = make((300, 40), torch.float32, torch.float32)
+    opt = AdamW([p])
+    opt.step()
+    before = [x.clone() for x in opt.moments()]
+    zeros, made = torch.zeros, []
+
+    def full(*args, **kw):
+        made.append(1)
+        if len(made) > call:
+            raise torch.OutOfMemoryError("no memory left")
+        return zeros(*args, **kw)
+    monkeypatch.setattr(torch, "zeros", full)
+    with pytest.raises(torch.OutOfMemoryError):
+        opt.add_param_group({"params": [q]})
+    monkeypatch.undo()
+    assert len(opt.param_groups) == 1 and q not in opt.state
+    assert all(torch.equal(a, b) for a, b in zip(opt.moments(), before))
+    opt.step()
+    assert int(opt.state[p]["step"]) == 2
+    opt.add_param_group({"params": [q]})
+    opt.step()
+    assert int(opt.state[p]["step"]) == 3 and int(opt.state[q]["step"]) == 1
