@@ -53,7 +53,8 @@ def _as_rows(t: torch.Tensor | None):
     """(t, row stride) of a tensor the library can read, copied only where it cannot be read as it is."""
     if t is None:
         return None, 0
-    t = t.resolve_neg()  # torch's lazily negated views hold the opposite in memory
+    if t.is_neg():  # lazily negated: memory holds the opposite
+        t = t.resolve_neg()
     stride = _row_stride(t)
     if stride is None:
         t = t.contiguous()
@@ -61,20 +62,14 @@ def _as_rows(t: torch.Tensor | None):
     return t, stride
 
 
-def _reading(logits, targets, mask, tau: float, topk: int):
-    """(parameters, logits, mask) of one call of the library: both tensors as it reads them, with their strides."""
+def _forward(logits, targets, mask, tau: float, topk: int, stats):
+    """(parameters, logprobs, entropy, lse, top_ids, top_logprobs); targets int64, contiguous; ``stats``
+    (fp32 [..., 2] or None) receives what the backward needs."""
+    lib, dev, lead = N.load(), logits.device, logits.shape[:-1]
     x, stride = _as_rows(logits)
     m, m_stride = _as_rows(mask)
-    p = N.LogprobParams(math.prod(logits.shape[:-1]), logits.shape[-1], stride, m_stride,
-                        targets.shape[-1] if targets.dim() == logits.dim() else 1, topk, tau, N.DTYPES[logits.dtype], 0)
-    return p, x, m
-
-
-def _forward(logits, targets, mask, tau: float, topk: int, stats):
-    """(logprobs, entropy, lse, top_ids, top_logprobs); targets int64, contiguous; ``stats`` (fp32 [..., 2] or
-    None) receives what the backward needs."""
-    lib, dev, lead = N.load(), logits.device, logits.shape[:-1]
-    p, x, m = _reading(logits, targets, mask, tau, topk)
+    p = N.LogprobParams(math.prod(lead), logits.shape[-1], stride, m_stride,
+                        targets.shape[-1] if targets.dim() > len(lead) else 1, topk, tau, N.DTYPES[logits.dtype], 0)
     logprobs = torch.empty_like(targets, dtype=torch.float32)
     entropy, lse = (torch.empty(lead, dtype=torch.float32, device=dev) for _ in range(2))
     top_logprobs = torch.empty((*lead, topk), dtype=torch.float32, device=dev)
@@ -86,21 +81,32 @@ def _forward(logits, targets, mask, tau: float, topk: int, stats):
                                         entropy.data_ptr(), lse.data_ptr(), top_ids.data_ptr(),
                                         top_logprobs.data_ptr(), N.ptr(stats), N.ptr(ws), need,
                                         N.error_word(dev).data_ptr(), N.stream_handle(dev)), "logprob_forward")
-    return logprobs, entropy, lse, top_ids, top_logprobs
+    return p, logprobs, entropy, lse, top_ids, top_logprobs
 
 
-def _kind(t: torch.Tensor | None):
-    return None if t is None else (t.shape, t.dtype, t.device)
+def _as_saved(p, device: int, logits, targets, mask, top_ids, entropy, stats) -> bool:
+    """Whether these are of the sizes, types and device that a backward with these parameters reads."""
+    rows, width = p.rows, p.width
+    if logits.shape[-1:] != (width,) or N.DTYPES.get(logits.dtype) != p.dtype:
+        return False
+    if mask is not None and (mask.shape[-1:] != (width,) or mask.numel() not in (rows * width, width)
+                             or mask.dtype is not torch.uint8 or mask.get_device() != device):
+        return False
+    for t, n, dtype in ((logits, rows * width, logits.dtype), (targets, rows * p.targets, torch.int64),
+                        (top_ids, rows * p.topk, torch.int64), (entropy, rows, torch.float32),
+                        (stats, 2 * rows, torch.float32)):
+        if t.numel() != n or t.dtype is not dtype or t.get_device() != device:
+            return False
+    return True
 
 
 class _TargetLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, mask, tau: float, topk: int):
         stats = torch.empty((*logits.shape[:-1], 2), dtype=torch.float32, device=logits.device)
-        logprobs, entropy, lse, top_ids, top_logprobs = _forward(logits, targets, mask, tau, topk, stats)
-        saved = logits, targets, mask, top_ids, entropy, stats
-        ctx.save_for_backward(*saved)
-        ctx.call, ctx.kinds = (tau, topk), tuple(map(_kind, saved))
+        p, logprobs, entropy, lse, top_ids, top_logprobs = _forward(logits, targets, mask, tau, topk, stats)
+        ctx.save_for_backward(logits, targets, mask, top_ids, entropy, stats)
+        ctx.call = p, logits.get_device()
         ctx.mark_non_differentiable(top_ids)
         ctx.set_materialize_grads(False)
         return logprobs, entropy, lse, top_ids, top_logprobs
@@ -108,15 +114,20 @@ class _TargetLogprobs(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, g_logprobs, g_entropy, g_lse, _g_ids, g_top):
-        saved = ctx.saved_tensors
-        # hooks on saved tensors (checkpointing, offloading) may hand back copies with other strides
-        if tuple(map(_kind, saved)) != ctx.kinds:
+        p, device = ctx.call
+        logits, targets, mask, top_ids, entropy, stats = saved = ctx.saved_tensors
+        # hooks on saved tensors (checkpointing, offloading) may hand back copies, with other strides
+        if not _as_saved(p, device, *saved):
             raise RuntimeError("target_logprobs: a saved tensor came back with another shape, type or device")
-        logits, _, mask = saved[:3]
-        targets, top_ids, entropy, stats = (t.contiguous() for t in (saved[1], *saved[3:]))
-        p, x, m = _reading(logits, targets, mask, *ctx.call)
+        x, stride = _as_rows(logits)
+        m, m_stride = _as_rows(mask)
+        if stride != p.row_stride or m_stride != p.mask_row_stride:
+            p = N.LogprobParams.from_buffer_copy(p)
+            p.row_stride, p.mask_row_stride = stride, m_stride
         dev = logits.device
-        ups = [g if g is None else g.resolve_neg().contiguous() for g in (g_logprobs, g_entropy, g_lse, g_top)]
+        targets, top_ids, entropy, stats = (t.contiguous() for t in (targets, top_ids, entropy, stats))
+        ups = [g if g is None else g.resolve_neg().contiguous() if g.is_neg() else g.contiguous()
+               for g in (g_logprobs, g_entropy, g_lse, g_top)]
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
         with N.on_device(dev):
             N.check(N.load().mkg_logprob_backward(p, x.data_ptr(), N.ptr(m), targets.data_ptr(),
@@ -179,4 +190,4 @@ def target_logprobs(logits: torch.Tensor, targets: torch.Tensor, tau: float = 1.
     m = None if mask is None else mask.view(torch.uint8)
     if logits.requires_grad and torch.is_grad_enabled():
         return TargetLogprobs(*_TargetLogprobs.apply(logits, t, m, tau, int(topk)))
-    return TargetLogprobs(*_forward(logits, t, m, tau, int(topk), None))
+    return TargetLogprobs(*_forward(logits, t, m, tau, int(topk), None)[1:])
