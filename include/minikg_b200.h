@@ -679,8 +679,8 @@ typedef struct mkg_adamw_state {
  * indexes into steps (each index at most once).  params are updated in place:
  *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,  t = its step count + 1,
  *   p = p (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
- * in fp32 (fp64 for moments in 8 bits, rounded once to what is held; the update takes m and v
- * before that rounding).  Gradients that are not finite make the values they meet NaN. */
+ * in fp32.  What 8 bits hold is m and v in fp64 rounded once (beyond the largest held value: that value); the
+ * update takes them in fp32, before that rounding.  Gradients that are not finite make the values they meet NaN. */
 int mkg_adamw_step(const mkg_adamw_params* p, const mkg_adamw_state* state, int64_t n, void* const* params,
                    const void* const* grads, const int64_t* numel, const int64_t* offset, const int64_t* index,
                    mkg_stream stream);

@@ -15,7 +15,7 @@
 // rounded once: rounding to fp32 first would move about one sum in 10^6 to the neighbouring value, and
 // with 16-bit gradients sums on the middle of two values are frequent (about one in 200).  The sums are
 // taken in fp32 with a bound on their error; where both ends of the interval round to the same code that
-// is the fp64 sum's code too, and only the others are taken again in fp64.
+// is the fp64 sum's code too, and only the others are taken again in fp64.  The update takes the fp32 sums.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>

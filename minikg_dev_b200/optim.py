@@ -9,7 +9,8 @@ a step can be captured in a CUDA graph (``proof.ProofRunner.capture(optimizer=..
 
 ``state_bits=8`` holds each moment in one byte and shares a power of two between 256 values: 2.03
 bytes a parameter in place of 8.  First moments have 4 significant bits, second moments 4 over 34
-binades; a second moment above 0 is never held as 0.  Sums are taken in fp64 and rounded once.
+binades; a second moment above 0 is never held as 0.  What is held is the sum in fp64 rounded once; the
+update takes the sum in fp32.
 """
 from __future__ import annotations
 
